@@ -123,6 +123,45 @@ typedef struct kcg_fmha_desc {
   int32_t reserved;
 } kcg_fmha_desc;
 
+/* Attention for training: the tensors are VIEWS of [B, heads, S, D] with any batch, head and row
+ * stride (in elements, in that order; every used stride positive and a multiple of 8, the entries of a
+ * row contiguous), so that queries, keys and values can be read out of a packed projection and their
+ * gradients written back into one.  Hkv key/value heads serve H query heads: query head h reads
+ * key/value head h / (H / Hkv).  The stride of an extent of one is not looked at.  Only KCG_BF16.
+ * causal: query i sees keys j <= i + (Skv - Sq), as in kcg_fmha_desc. */
+typedef struct kcg_attn_desc {
+  int32_t B, H, Hkv;
+  int32_t Sq, Skv;
+  int32_t D;          /* head dim: 64 or 128 */
+  int32_t dtype;      /* kcg_dtype_t of every tensor but lse */
+  int32_t causal;
+  float scale;        /* multiplies the logits before exp, > 0 */
+  int32_t reserved;
+  int64_t q[3], k[3], v[3], o[3];        /* strides of Q, K, V, O */
+  int64_t d_o[3], d_q[3], d_k[3], d_v[3]; /* strides of the gradients (backward only) */
+} kcg_attn_desc;
+
+/* Norm and position rotation of queries and keys: views of [B, heads, S, D] as in kcg_attn_desc, but of
+ * KCG_F32 or KCG_BF16 and with any non-negative strides (16-byte rows and R a multiple of two 16-byte
+ * vectors take the fast path).  H query heads and Hk key heads (0: no keys) of the same tokens. */
+typedef struct kcg_rope_desc {
+  int32_t B, S;
+  int32_t H, Hk;
+  int32_t D;           /* entries of a head, even, at most 256 */
+  int32_t R;           /* entries that are rotated, even, at most D */
+  int32_t dtype;       /* kcg_dtype_t of queries, keys and their gradients */
+  int32_t dtype_w;     /* kcg_dtype_t of the norm weights */
+  int32_t interleaved; /* pairs: 0 = (i, i + R/2), 1 = (2i, 2i + 1) */
+  int32_t pos_bits;    /* 32 or 64: signed integer type of the positions */
+  int64_t table_rows;  /* rows of the cos and sin tables */
+  float eps;           /* added to the mean square, >= 0 */
+  int32_t reserved;
+  int64_t pos[2];      /* strides of the positions: batch, token (0 allowed) */
+  int64_t q[3], k[3];          /* strides of the inputs: batch, head, row */
+  int64_t q_out[3], k_out[3];  /* of the outputs, and of the gradients that come back for them */
+  int64_t d_q[3], d_k[3];      /* of the inputs' gradients (backward only) */
+} kcg_rope_desc;
+
 /* Scratch the launch can use (bytes; may be 0).
  * GEMM: (1) required for 3xTF32: the fp32 residuals (x minus its TF32 truncation) of A and B,
  * 4*(M*K + K*N) bytes, each array rounded up to 256; (2) optional, behind (1), for launches on
@@ -194,6 +233,47 @@ kcg_status_t kcg_gemm_launch_static(const kcg_gemm_desc* d, const void* A, const
 kcg_status_t kcg_fmha_fwd_launch(const kcg_fmha_desc* d, const void* Q, const void* K,
                                  const void* V, void* O, void* workspace, size_t workspace_bytes,
                                  void* stream);
+
+/* Attention forward that also leaves what its gradient needs: O as above and
+ * lse[b, h, i] = log sum_j exp(scale * q_i.k_j) over the visible keys (fp32, contiguous [B, H, Sq],
+ * natural logarithm; -inf and O = 0 for a query that sees no key).  No counterpart in the reference,
+ * which generates forward kernels only. */
+kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
+                                     float* lse, void* stream);
+
+/* Its gradients, from the gradient of O and the O and lse of that forward call (no probabilities are
+ * kept; they are recomputed tile by tile):
+ *   P_ij = exp(scale q_i.k_j - lse_i), delta_i = dO_i.O_i, dS_ij = P_ij (dO_i.v_j - delta_i),
+ *   dV_j = sum_i P_ij dO_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j,
+ * the sums of dK and dV over all query heads of the group.  Accumulation in fp32 in a fixed order (the
+ * same bits on every call).  The outputs must not overlap one another or an input; the inputs must be
+ * finite wherever the tensors have an entry (a masked NaN still reaches the products it is part of).
+ * Workspace: kcg_fmha_bwd_workspace_bytes, not shared by calls that may overlap. */
+size_t kcg_fmha_bwd_workspace_bytes(const kcg_attn_desc* d);
+kcg_status_t kcg_fmha_bwd_launch(const kcg_attn_desc* d, const void* dO, const void* Q, const void* K, const void* V,
+                                 const void* O, const float* lse, void* dQ, void* dK, void* dV, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* For every head row x of queries and keys: n = x / sqrt(mean(x^2) + eps) * weight (weight [D] for all
+ * query heads, another for all key heads; NULL = ones), and the pairs (a, b) of its first R entries
+ * rotated: (a cos - b sin, b cos + a sin), with the row positions[b, s] of the tables cos, sin (fp32,
+ * contiguous [table_rows, R/2]; positions NULL = s).  Computed in fp32, rounded once.  A position
+ * outside the tables gives NaN in the rotated entries and code 11 in the status word
+ * (kcg_last_device_status); nothing is read there.  An output may be the same view as its input.  No
+ * counterpart in the reference. */
+kcg_status_t kcg_qk_norm_rope_launch(const kcg_rope_desc* d, const void* q, const void* k, const void* q_weight,
+                                     const void* k_weight, const void* cos, const void* sin, const void* positions,
+                                     void* q_out, void* k_out, void* stream);
+
+/* Its gradients, from those of the outputs and the inputs of the forward call: dq, dk (which may be the
+ * same views as dq_out, dk_out or as q, k), and the weights' [D] in fp32 (dq_weight / dk_weight NULL =
+ * not wanted; otherwise the workspace of kcg_qk_norm_rope_bwd_workspace_bytes, not shared by calls that
+ * may overlap).  Sums in a fixed order. */
+size_t kcg_qk_norm_rope_bwd_workspace_bytes(const kcg_rope_desc* d);
+kcg_status_t kcg_qk_norm_rope_bwd_launch(const kcg_rope_desc* d, const void* dq_out, const void* dk_out, const void* q,
+                                         const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                                         const void* sin, const void* positions, void* dq, void* dk, float* dq_weight,
+                                         float* dk_weight, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The reference's Softmax operator on its own (src/Frontend/Operators.cc:474-536): last-axis
  * exp(x)/sum(exp(x)) over a [rows, cols] fp32 array, in place when y == x.  Used for graphs

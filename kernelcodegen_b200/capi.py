@@ -41,6 +41,12 @@ EXPORTED_SYMBOLS = (
     "kcg_gemm_launch",
     "kcg_gemm_launch_static",
     "kcg_fmha_fwd_launch",
+    "kcg_fmha_fwd_lse_launch",
+    "kcg_fmha_bwd_workspace_bytes",
+    "kcg_fmha_bwd_launch",
+    "kcg_qk_norm_rope_launch",
+    "kcg_qk_norm_rope_bwd_workspace_bytes",
+    "kcg_qk_norm_rope_bwd_launch",
     "kcg_softmax_launch",
     "kcg_batched_gemm_launch",
     "kcg_batched_gemm_workspace_bytes",
@@ -95,6 +101,29 @@ class FmhaDesc(Structure):
     ]
 
 
+class AttnDesc(Structure):
+    """Mirror of `struct kcg_attn_desc`."""
+
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("Hkv", c_int32), ("Sq", c_int32), ("Skv", c_int32), ("D", c_int32),
+        ("dtype", c_int32), ("causal", c_int32), ("scale", c_float), ("reserved", c_int32),
+        ("q", c_int64 * 3), ("k", c_int64 * 3), ("v", c_int64 * 3), ("o", c_int64 * 3),
+        ("d_o", c_int64 * 3), ("d_q", c_int64 * 3), ("d_k", c_int64 * 3), ("d_v", c_int64 * 3),
+    ]
+
+
+class RopeDesc(Structure):
+    """Mirror of `struct kcg_rope_desc`."""
+
+    _fields_ = [
+        ("B", c_int32), ("S", c_int32), ("H", c_int32), ("Hk", c_int32), ("D", c_int32), ("R", c_int32),
+        ("dtype", c_int32), ("dtype_w", c_int32), ("interleaved", c_int32), ("pos_bits", c_int32),
+        ("table_rows", c_int64), ("eps", c_float), ("reserved", c_int32), ("pos", c_int64 * 2),
+        ("q", c_int64 * 3), ("k", c_int64 * 3), ("q_out", c_int64 * 3), ("k_out", c_int64 * 3),
+        ("d_q", c_int64 * 3), ("d_k", c_int64 * 3),
+    ]
+
+
 class KcgError(RuntimeError):
     def __init__(self, status: int, what: str):
         self.status = status
@@ -136,6 +165,18 @@ def load() -> ctypes.CDLL:
     lib.kcg_gemm_launch_static.argtypes = [POINTER(GemmDesc), c_void_p, c_void_p, c_void_p, c_void_p]
     lib.kcg_fmha_fwd_launch.restype = c_int
     lib.kcg_fmha_fwd_launch.argtypes = [POINTER(FmhaDesc), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.kcg_fmha_fwd_lse_launch.restype = c_int
+    lib.kcg_fmha_fwd_lse_launch.argtypes = [POINTER(AttnDesc), *[c_void_p] * 6]
+    lib.kcg_fmha_bwd_workspace_bytes.restype = c_size_t
+    lib.kcg_fmha_bwd_workspace_bytes.argtypes = [POINTER(AttnDesc)]
+    lib.kcg_fmha_bwd_launch.restype = c_int
+    lib.kcg_fmha_bwd_launch.argtypes = [POINTER(AttnDesc), *[c_void_p] * 10, c_size_t, c_void_p]
+    lib.kcg_qk_norm_rope_launch.restype = c_int
+    lib.kcg_qk_norm_rope_launch.argtypes = [POINTER(RopeDesc), *[c_void_p] * 10]
+    lib.kcg_qk_norm_rope_bwd_workspace_bytes.restype = c_size_t
+    lib.kcg_qk_norm_rope_bwd_workspace_bytes.argtypes = [POINTER(RopeDesc)]
+    lib.kcg_qk_norm_rope_bwd_launch.restype = c_int
+    lib.kcg_qk_norm_rope_bwd_launch.argtypes = [POINTER(RopeDesc), *[c_void_p] * 14, c_size_t, c_void_p]
     lib.kcg_softmax_launch.restype = c_int
     lib.kcg_softmax_launch.argtypes = [c_int64, c_int64, c_void_p, c_void_p, c_void_p]
     lib.kcg_batched_gemm_launch.restype = c_int

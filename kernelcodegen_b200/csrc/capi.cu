@@ -127,6 +127,30 @@ kcg_status_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, con
   return KCG_OK;
 }
 
+kcg_status_t check_head_view(const HeadView& v, int elem_bytes) {
+  if (!aligned16(v.base)) return KCG_BAD_ALIGN;
+  const int64_t s[3] = {v.sr, v.sh, v.sb};
+  const int n[3] = {v.S, v.H, v.B};
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] == 1) continue;
+    if (s[i] <= 0 || s[i] > (int64_t{1} << 39) / elem_bytes) return KCG_BAD_SHAPE;
+    if (s[i] * elem_bytes % 16) return KCG_BAD_ALIGN;
+  }
+  return KCG_OK;
+}
+
+kcg_status_t encode_head_view(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const HeadView& v,
+                              CUtensorMapSwizzle swizzle) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(v.D), static_cast<uint64_t>(v.S), static_cast<uint64_t>(v.H),
+                            static_cast<uint64_t>(v.B)};
+  const uint64_t row = static_cast<uint64_t>(v.D) * elem_bytes;
+  const uint64_t strides[3] = {v.S == 1 ? row : static_cast<uint64_t>(v.sr) * elem_bytes,
+                               v.H == 1 ? row : static_cast<uint64_t>(v.sh) * elem_bytes,
+                               v.B == 1 ? row : static_cast<uint64_t>(v.sb) * elem_bytes};
+  const uint32_t box[4] = {128u / static_cast<uint32_t>(elem_bytes), 128, 1, 1};
+  return encode_tmap(map, dt, 4, v.base, dims, strides, box, swizzle);
+}
+
 // One thread waits on an mbarrier that nothing ever arrives on: exercises the bounded wait the
 // kernels use (iteration cap -> status word -> clean return) without involving any other unit.
 __global__ void selftest_wait_kernel(int* status, uint32_t limit) {
@@ -200,6 +224,37 @@ kcg_status_t kcg_fmha_fwd_launch(const kcg_fmha_desc* d, const void* Q, const vo
                                  void* stream) {
   return fmha_launch_impl(d, Q, K, V, O, workspace, workspace_bytes,
                           static_cast<cudaStream_t>(stream));
+}
+
+kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
+                                     float* lse, void* stream) {
+  return fmha_lse_launch_impl(d, Q, K, V, O, lse, static_cast<cudaStream_t>(stream));
+}
+
+size_t kcg_fmha_bwd_workspace_bytes(const kcg_attn_desc* d) { return fmha_bwd_workspace_impl(d); }
+
+kcg_status_t kcg_fmha_bwd_launch(const kcg_attn_desc* d, const void* dO, const void* Q, const void* K, const void* V,
+                                 const void* O, const float* lse, void* dQ, void* dK, void* dV, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  return fmha_bwd_launch_impl(d, dO, Q, K, V, O, lse, dQ, dK, dV, workspace, workspace_bytes,
+                              static_cast<cudaStream_t>(stream));
+}
+
+kcg_status_t kcg_qk_norm_rope_launch(const kcg_rope_desc* d, const void* q, const void* k, const void* q_weight,
+                                     const void* k_weight, const void* cos, const void* sin, const void* positions,
+                                     void* q_out, void* k_out, void* stream) {
+  return qk_norm_rope_impl(d, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out,
+                           static_cast<cudaStream_t>(stream));
+}
+
+size_t kcg_qk_norm_rope_bwd_workspace_bytes(const kcg_rope_desc* d) { return qk_norm_rope_bwd_workspace_impl(d); }
+
+kcg_status_t kcg_qk_norm_rope_bwd_launch(const kcg_rope_desc* d, const void* dq_out, const void* dk_out, const void* q,
+                                         const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                                         const void* sin, const void* positions, void* dq, void* dk, float* dq_weight,
+                                         float* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+  return qk_norm_rope_bwd_impl(d, dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, dq, dk, dq_weight,
+                               dk_weight, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 kcg_status_t kcg_gemm_host(const kcg_gemm_desc* d, const void* hA, const void* hB, void* hC) {

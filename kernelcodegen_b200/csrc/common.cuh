@@ -30,6 +30,24 @@ kcg_status_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, con
                          const uint32_t* box,
                          CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
+// Tensor map of a [B, H, S, D] view (strides in elements; the innermost is 1): coordinates
+// (d, row, head, batch), boxes of 128 rows x 128 bytes, rows past S read as zero.  An extent of one
+// has no stride of its own; it is given one that the encoder accepts.
+struct HeadView {
+  const void* base;
+  int B, H, S, D;
+  int64_t sb, sh, sr;
+};
+kcg_status_t encode_head_view(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const HeadView& v,
+                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+// Whether a view can be read through such a map (16-byte rows) or written row by row.
+kcg_status_t check_head_view(const HeadView& v, int elem_bytes);
+// bytes from the first to one past the last element
+inline unsigned long long head_view_extent(const HeadView& v, int elem_bytes) {
+  return (static_cast<unsigned long long>(v.B - 1) * v.sb + static_cast<unsigned long long>(v.H - 1) * v.sh +
+          static_cast<unsigned long long>(v.S - 1) * v.sr + v.D) * elem_bytes;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 #define KCG_CUDA_TRY(expr)                                                        \
@@ -63,6 +81,21 @@ kcg_status_t gemm_host_staged_impl(const kcg_gemm_desc* d, const void* hA, const
 kcg_status_t fmha_launch_impl(const kcg_fmha_desc* d, const void* Q, const void* K, const void* V,
                               void* O, void* ws, size_t ws_bytes, cudaStream_t stream);
 size_t fmha_workspace_impl(const kcg_fmha_desc* d);
+kcg_status_t attn_check_desc(const kcg_attn_desc* d);
+kcg_status_t fmha_lse_launch_impl(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
+                                  float* lse, cudaStream_t stream);
+size_t fmha_bwd_workspace_impl(const kcg_attn_desc* d);
+kcg_status_t fmha_bwd_launch_impl(const kcg_attn_desc* d, const void* dO, const void* Q, const void* K, const void* V,
+                                  const void* O, const float* lse, void* dQ, void* dK, void* dV, void* ws,
+                                  size_t ws_bytes, cudaStream_t stream);
+kcg_status_t qk_norm_rope_impl(const kcg_rope_desc* d, const void* q, const void* k, const void* wq, const void* wk,
+                               const void* cs, const void* sn, const void* pos, void* q_out, void* k_out,
+                               cudaStream_t stream);
+size_t qk_norm_rope_bwd_workspace_impl(const kcg_rope_desc* d);
+kcg_status_t qk_norm_rope_bwd_impl(const kcg_rope_desc* d, const void* dq_out, const void* dk_out, const void* q,
+                                   const void* k, const void* wq, const void* wk, const void* cs, const void* sn,
+                                   const void* pos, void* dq, void* dk, float* dwq, float* dwk, void* ws,
+                                   size_t ws_bytes, cudaStream_t stream);
 kcg_status_t softmax_launch_impl(long long rows, long long cols, const void* x, void* y, cudaStream_t stream);
 
 }  // namespace kcg

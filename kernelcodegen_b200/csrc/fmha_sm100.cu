@@ -48,7 +48,10 @@ constexpr int BKV = 128;       // keys per block
 
 struct FmhaParams {
   void* O;
+  int H, group;      // query heads, query heads per key/value head
   int Sq, Skv;
+  long long o_sb, o_sh, o_sr;  // strides of O in elements
+  float* lse;        // [B, H, Sq] log-sum-exp of every row's scaled scores (LSE instantiations)
   int causal;
   int out_bf16;
   float scale_log2;  // scale * log2(e)
@@ -94,19 +97,20 @@ __device__ __forceinline__ void reg_alloc_200() {
 // Measured: with head dimension 64 in bf16 the tensor core needs half as long per block as the
 // MUFU unit and a share of 3/8 gains 9 %; with head dimension 128, or TF32 operands, the two
 // are level and any share costs 1-9 %.
-template <int POLY>
+// FINE: the quartic, where the row sum is kept (its logarithm is an fp32 result).
+template <int POLY, bool FINE>
 __device__ __forceinline__ float2 exp2_pair(int g, int pi, float2 x) {
   if (((pi * 5 + g * 3) & 7) < POLY) {
     x.x = fmaxf(x.x, -125.f);   // masked keys (-inf) and far tails end as 2^-125, nothing in the sums
     x.y = fmaxf(x.y, -125.f);
-    return ex2_poly2(x);
+    return FINE ? ex2_quartic2(x) : ex2_poly2(x);
   }
   x.x = ex2_approx(x.x);
   x.y = ex2_approx(x.y);
   return x;
 }
 
-template <int D, bool TF>
+template <int D, bool TF, bool LSE>
 __global__ void __launch_bounds__(FM_THREADS, 1)
 fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const FmhaParams p) {
@@ -163,6 +167,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
   g0 += grp * gsz;
   const int rem = idx - grp * gsz * p.n_qp;
   const int bh = g0 + rem % gsz;
+  const int b = bh / p.H, h = bh - b * p.H, hk = h / p.group;
   const int qpair = p.causal ? (p.n_qp - 1 - rem / gsz) : (rem / gsz);
   const int q0 = qpair * (QTILES * BQ);
   const int shift = p.Skv - p.Sq;  // causal: query i sees keys j <= i + shift
@@ -207,14 +212,14 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         mbar_expect_tx(bar_q + 8 * t, TILE);
 #pragma unroll
         for (int dp = 0; dp < DPANELS; ++dp)
-          tma_load_3d(sQ + t * TILE + dp * PANEL, &tmQ, bar_q + 8 * t, dp * PW, q0 + t * BQ, bh);
+          tma_load_4d(sQ + t * TILE + dp * PANEL, &tmQ, bar_q + 8 * t, dp * PW, q0 + t * BQ, h, b);
       }
       mbar_expect_tx(bar_kfull, TILE);
 #pragma unroll
-      for (int dp = 0; dp < DPANELS; ++dp) tma_load_3d(sK + dp * PANEL, &tmK, bar_kfull, dp * PW, 0, bh);
+      for (int dp = 0; dp < DPANELS; ++dp) tma_load_4d(sK + dp * PANEL, &tmK, bar_kfull, dp * PW, 0, hk, b);
       mbar_expect_tx(bar_vfull, TILE);
 #pragma unroll
-      for (int dp = 0; dp < DPANELS; ++dp) tma_load_3d(sV + dp * PANEL, &tmV, bar_vfull, dp * PW, 0, bh);
+      for (int dp = 0; dp < DPANELS; ++dp) tma_load_4d(sV + dp * PANEL, &tmV, bar_vfull, dp * PW, 0, hk, b);
     }
   }
   if (warp == 1) {
@@ -233,20 +238,20 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       // (block 0 and the Q tiles were issued before the CTA-wide synchronisation above)
       bool ok = true;
       for (int j = 1; j < n_kv && ok; ++j) {
-        const int b = j & 1;
+        const int st = j & 1;
         const uint32_t par = ((j >> 1) & 1u) ^ 1u;
-        ok = mbar_wait(bar_kempty + 8 * b, par, abort_flag, p.status, DEV_TIMEOUT_PRODUCER, p.spin);
+        ok = mbar_wait(bar_kempty + 8 * st, par, abort_flag, p.status, DEV_TIMEOUT_PRODUCER, p.spin);
         if (!ok) break;
-        mbar_expect_tx(bar_kfull + 8 * b, TILE);
+        mbar_expect_tx(bar_kfull + 8 * st, TILE);
 #pragma unroll
         for (int dp = 0; dp < DPANELS; ++dp)
-          tma_load_3d(sK + b * TILE + dp * PANEL, &tmK, bar_kfull + 8 * b, dp * PW, j * BKV, bh);
-        ok = mbar_wait(bar_vempty + 8 * b, par, abort_flag, p.status, DEV_TIMEOUT_PRODUCER, p.spin);
+          tma_load_4d(sK + st * TILE + dp * PANEL, &tmK, bar_kfull + 8 * st, dp * PW, j * BKV, hk, b);
+        ok = mbar_wait(bar_vempty + 8 * st, par, abort_flag, p.status, DEV_TIMEOUT_PRODUCER, p.spin);
         if (!ok) break;
-        mbar_expect_tx(bar_vfull + 8 * b, TILE);
+        mbar_expect_tx(bar_vfull + 8 * st, TILE);
 #pragma unroll
         for (int dp = 0; dp < DPANELS; ++dp)
-          tma_load_3d(sV + b * TILE + dp * PANEL, &tmV, bar_vfull + 8 * b, dp * PW, j * BKV, bh);
+          tma_load_4d(sV + st * TILE + dp * PANEL, &tmV, bar_vfull + 8 * st, dp * PW, j * BKV, hk, b);
       }
       if (!ok) {
         // give copies already in flight time to land before shared memory is released
@@ -328,7 +333,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (ok && elect_one()) umma_commit(bar_kempty);  // K_0 is free once S_0(0), S_1(0) have read it
       __syncwarp();
       for (int j = 0; j < n_kv && ok; ++j) {
-        const int b = j & 1;
+        const int st = j & 1;
         const uint32_t par = (j >> 1) & 1u;
         const bool next = j + 1 < n_kv;
         bool k_next_ready = false;
@@ -336,7 +341,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         for (int t = 0; t < QTILES && ok; ++t) {
           if (j < n_kv_t[t]) {
             if (t == 0 || j >= n_kv_t[0]) {
-              ok = wait_all(bar_vfull + 8 * b, par, DEV_TIMEOUT_MMA_FULL);
+              ok = wait_all(bar_vfull + 8 * st, par, DEV_TIMEOUT_MMA_FULL);
               if (!ok) break;
             }
             ok = wait_all(bar_pfull + 8 * t, j & 1u, DEV_TIMEOUT_P);
@@ -346,7 +351,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           }
           if (next && j + 1 < n_kv_t[t]) {
             if (!k_next_ready) {
-              ok = wait_all(bar_kfull + 8 * (b ^ 1), ((j + 1) >> 1) & 1u, DEV_TIMEOUT_MMA_FULL);
+              ok = wait_all(bar_kfull + 8 * (st ^ 1), ((j + 1) >> 1) & 1u, DEV_TIMEOUT_MMA_FULL);
               if (!ok) break;
               k_next_ready = true;
               tc_fence_after();
@@ -356,8 +361,8 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
         if (!ok) break;
         if (elect_one()) {
-          umma_commit(bar_vempty + 8 * b);
-          if (next) umma_commit(bar_kempty + 8 * (b ^ 1));
+          umma_commit(bar_vempty + 8 * st);
+          if (next) umma_commit(bar_kempty + 8 * (st ^ 1));
         }
         __syncwarp();
       }
@@ -452,7 +457,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
           for (int i = 0; i < 32; i += 2) {
             float2 x = fma2(make_float2(__uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1])), make_float2(c, c),
                             make_float2(-mc, -mc));
-            x = exp2_pair<POLY>(g, i >> 1, x);
+            x = exp2_pair<POLY, LSE>(g, i >> 1, x);
             rsg[(i >> 1) & 3] = add2(rsg[(i >> 1) & 3], x);
             sr[g][i] = __float_as_uint(x.x);
             sr[g][i + 1] = __float_as_uint(x.y);
@@ -469,7 +474,7 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             for (int i = 0; i < 32; i += 2) {
               float2 x = fma2(make_float2(__uint_as_float(sr[2 * hh + g][i]), __uint_as_float(sr[2 * hh + g][i + 1])),
                               make_float2(c, c), make_float2(-mc, -mc));
-              x = exp2_pair<POLY>(2 * hh + g, i >> 1, x);
+              x = exp2_pair<POLY, LSE>(2 * hh + g, i >> 1, x);
               rsg[(i >> 1) & 3] = add2(rsg[(i >> 1) & 3], x);
               pk[16 * g + (i >> 1)] = pack_bf16x2(x.x, x.y);
             }
@@ -500,11 +505,12 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         tc_fence_before();
       }
     }
-    const size_t off = (static_cast<size_t>(bh) * p.Sq + row) * D;
+    const size_t off = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(h) * p.o_sh + static_cast<size_t>(row) * p.o_sr;
     if (ok && row < p.Sq &&
         bounds_ok(off * (p.out_bf16 ? 2 : 4), static_cast<unsigned long long>(D) * (p.out_bf16 ? 2 : 4), p.o_extent,
                   p.status, p.bounds_detail)) {
       const float inv = l > 1e-30f ? 1.f / l : 0.f;   // a row with no visible key sums to < 2^-100
+      if (LSE) p.lse[static_cast<size_t>(bh) * p.Sq + row] = l > 1e-30f ? (m * c + __log2f(l)) * 0.6931471805599453f : -INFINITY;
       if (p.out_bf16) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.O) + off);
 #pragma unroll
@@ -583,12 +589,12 @@ __global__ void __launch_bounds__(256) f32_to_bf16_kernel(CastArgs a) {
 
 inline size_t pad256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-template <int D, bool TF = false>
+template <int D, bool TF = false, bool LSE = false>
 kcg_status_t launch_fmha(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                          const FmhaParams& p, int bh, cudaStream_t stream, bool after_cast) {
   using Cfg = FmhaCfg<D, TF>;
   static_assert(Cfg::SMEM_TOTAL <= 232448, "shared memory budget");
-  auto kern = fmha_fwd_kernel<D, TF>;
+  auto kern = fmha_fwd_kernel<D, TF, LSE>;
   KCG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     Cfg::SMEM_TOTAL));
   FmhaParams pp = p;
@@ -696,31 +702,27 @@ kcg_status_t fmha_launch_impl(const kcg_fmha_desc* d, const void* Q, const void*
   }
   CUtensorMap tq, tk, tv;
   // one 128-byte swizzle panel of a tile per copy: 64 bf16 or 32 fp32 wide, 128 rows
-  const uint32_t box[3] = {tf ? 32u : 64u, 128, 1};
   const CUtensorMapDataType dt = tf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint64_t es = tf ? 4 : 2;
+  const int es = tf ? 4 : 2;
   // fp32 V is an MN-major operand: 32-byte-atom form of the 128B swizzle
   const CUtensorMapSwizzle sw_v = tf ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B;
   {
-    const uint64_t dims[3] = {static_cast<uint64_t>(d->D), static_cast<uint64_t>(d->Sq),
-                              static_cast<uint64_t>(bh)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(d->D) * es,
-                                 static_cast<uint64_t>(d->Sq) * d->D * es};
-    kcg_status_t st = encode_tmap(&tq, dt, 3, q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (st != KCG_OK) return st;
-  }
-  {
-    const uint64_t dims[3] = {static_cast<uint64_t>(d->D), static_cast<uint64_t>(d->Skv),
-                              static_cast<uint64_t>(bh)};
-    const uint64_t strides[2] = {static_cast<uint64_t>(d->D) * es,
-                                 static_cast<uint64_t>(d->Skv) * d->D * es};
-    kcg_status_t st = encode_tmap(&tk, dt, 3, k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (st != KCG_OK) return st;
-    st = encode_tmap(&tv, dt, 3, v, dims, strides, box, sw_v);
+    auto view = [&](const void* x, int S) {
+      return HeadView{x, d->B, d->H, S, d->D, static_cast<int64_t>(d->H) * S * d->D, static_cast<int64_t>(S) * d->D, d->D};
+    };
+    kcg_status_t st = encode_head_view(&tq, dt, es, view(q, d->Sq));
+    if (st == KCG_OK) st = encode_head_view(&tk, dt, es, view(k, d->Skv));
+    if (st == KCG_OK) st = encode_head_view(&tv, dt, es, view(v, d->Skv), sw_v);
     if (st != KCG_OK) return st;
   }
   FmhaParams p;
   p.O = O;
+  p.lse = nullptr;
+  p.H = d->H;
+  p.group = 1;
+  p.o_sb = static_cast<long long>(d->H) * d->Sq * d->D;
+  p.o_sh = static_cast<long long>(d->Sq) * d->D;
+  p.o_sr = d->D;
   p.Sq = d->Sq;
   p.Skv = d->Skv;
   p.causal = d->causal ? 1 : 0;
@@ -737,6 +739,60 @@ kcg_status_t fmha_launch_impl(const kcg_fmha_desc* d, const void* Q, const void*
   if (tf) return launch_fmha<64, true>(tq, tk, tv, p, bh, stream, false);
   if (d->D == 64) return launch_fmha<64>(tq, tk, tv, p, bh, stream, false);
   return launch_fmha<128>(tq, tk, tv, p, bh, stream, d->dtype_in == KCG_F32);
+}
+
+kcg_status_t attn_check_desc(const kcg_attn_desc* d) {
+  if (!d) return KCG_BAD_ARGUMENT;
+  if (d->B <= 0 || d->H <= 0 || d->Hkv <= 0 || d->Sq <= 0 || d->Skv <= 0) return KCG_BAD_SHAPE;
+  if (d->D != 64 && d->D != 128) return KCG_BAD_SHAPE;
+  if (d->H % d->Hkv) return KCG_BAD_SHAPE;
+  if (static_cast<long long>(d->B) * d->H > 0x7FFFFFll) return KCG_BAD_SHAPE;
+  // row indexes are 32 bits, tiles of 256 rows past the end included
+  if (d->Sq > 0x7FFFFC00 || d->Skv > 0x7FFFFC00) return KCG_BAD_SHAPE;
+  if (d->dtype != KCG_BF16) return KCG_UNSUPPORTED;
+  if (!(d->scale > 0.f) || d->scale > 3.0e38f) return KCG_BAD_ARGUMENT;
+  return KCG_OK;
+}
+
+kcg_status_t fmha_lse_launch_impl(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
+                                  float* lse, cudaStream_t stream) {
+  kcg_status_t st = attn_check_desc(d);
+  if (st != KCG_OK) return st;
+  if (!Q || !K || !V || !O || !lse) return KCG_BAD_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return KCG_BAD_ALIGN;
+  const HeadView vq{Q, d->B, d->H, d->Sq, d->D, d->q[0], d->q[1], d->q[2]};
+  const HeadView vk{K, d->B, d->Hkv, d->Skv, d->D, d->k[0], d->k[1], d->k[2]};
+  const HeadView vv{V, d->B, d->Hkv, d->Skv, d->D, d->v[0], d->v[1], d->v[2]};
+  const HeadView vo{O, d->B, d->H, d->Sq, d->D, d->o[0], d->o[1], d->o[2]};
+  for (const HeadView* v : {&vq, &vk, &vv, &vo})
+    if ((st = check_head_view(*v, 2)) != KCG_OK) return st;
+  CUtensorMap tq, tk, tv;
+  if ((st = encode_head_view(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vq)) != KCG_OK) return st;
+  if ((st = encode_head_view(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vk)) != KCG_OK) return st;
+  if ((st = encode_head_view(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vv)) != KCG_OK) return st;
+  FmhaParams p;
+  p.O = O;
+  p.lse = lse;
+  p.H = d->H;
+  p.group = d->H / d->Hkv;
+  p.o_sb = d->B == 1 ? 0 : d->o[0];
+  p.o_sh = d->H == 1 ? 0 : d->o[1];
+  p.o_sr = d->Sq == 1 ? 0 : d->o[2];
+  p.Sq = d->Sq;
+  p.Skv = d->Skv;
+  p.causal = d->causal ? 1 : 0;
+  p.out_bf16 = 1;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.o_extent = head_view_extent(HeadView{O, d->B, d->H, d->Sq, d->D, p.o_sb, p.o_sh, p.o_sr}, 2);
+  if (const unsigned long long cap = debug_extent_limit()) p.o_extent = p.o_extent < cap ? p.o_extent : cap;
+  p.bounds_detail = nullptr;
+  debug_bounds_detail_ptr(&p.bounds_detail);
+  if ((st = device_status_ptr(&p.status)) != KCG_OK) return st;
+  const uint32_t spin = g_spin_limit.load();
+  p.spin = spin ? spin : KCG_SPIN_LIMIT;
+  const int bh = d->B * d->H;
+  if (d->D == 64) return launch_fmha<64, false, true>(tq, tk, tv, p, bh, stream, false);
+  return launch_fmha<128, false, true>(tq, tk, tv, p, bh, stream, false);
 }
 
 }  // namespace kcg

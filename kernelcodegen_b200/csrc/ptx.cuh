@@ -23,6 +23,7 @@ enum DeviceStatus : int {
   DEV_TIMEOUT_Q = 8,          // MMA issuer waited too long for the Q tile
   DEV_TIMEOUT_PEER = 9,       // a rank's completion flag did not arrive in time (kcg_peer_wait_launch)
   DEV_BOUNDS = 10,            // bounds-checking build: a store or a scratch access fell outside its buffer
+  DEV_BAD_POSITION = 11,      // a token's position lies outside the rotation tables
 };
 
 // Bounds-checking build (-DKCG_DEBUG_BOUNDS; the sanitizer tools are not available everywhere): every
@@ -169,6 +170,21 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
@@ -431,6 +447,33 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   r.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
   r.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
   return r;
+}
+
+// The same with a quartic for 2^f (relative error 2.6e-6): for sums and probabilities that are kept
+// or subtracted in 32 bits (saved row statistics, the backward pass).  Same clamp as ex2_poly2.
+__device__ __forceinline__ float2 ex2_quartic2(float2 x) {
+  constexpr float MAGIC = 12582912.f;
+  const float2 t = add2(x, make_float2(MAGIC, MAGIC));
+  const float2 n = add2(t, make_float2(-MAGIC, -MAGIC));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(f, make_float2(0.0095701f, 0.0095701f), make_float2(0.05591786f, 0.05591786f));
+  p = fma2(p, f, make_float2(0.24024745f, 0.24024745f));
+  p = fma2(p, f, make_float2(0.69312181f, 0.69312181f));
+  p = fma2(p, f, make_float2(0.99999926f, 0.99999926f));
+  float2 r;
+  r.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+  r.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+  return r;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t pa, pb, pd;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(pa) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(pb) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(pd) : "l"(pa), "l"(pb));
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(pd));
+  return d;
 }
 
 }  // namespace kcg

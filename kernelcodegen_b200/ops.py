@@ -200,6 +200,229 @@ def fmha(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float = 1.
     return out
 
 
+def _strides(t: torch.Tensor):
+    """Batch, head and row stride of a [B, H, S, D] view, as the C-ABI takes them."""
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _check_heads(name: str, t: torch.Tensor, shape: Sequence[int], dtype: torch.dtype, dev: torch.device) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != dev:
+        raise RuntimeError("all tensors must live on the same device")
+    if t.shape[3] != 1 and t.stride(3) != 1:
+        raise ValueError(f"{name} must have stride 1 in the last dimension")
+
+
+def _attn_desc(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool) -> "capi.AttnDesc":
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("expected Q [B,H,Sq,D] and K, V [B,Hkv,Skv,D]")
+    if q.dtype != torch.bfloat16 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("Q, K, V must be bfloat16: the gradients' contractions have no float32 form")
+    for name, t in (("Q", q), ("K", k), ("V", v)):
+        _check_heads(name, t, t.shape, q.dtype, q.device)
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("the number of query heads must be a multiple of the number of key/value heads")
+    d = capi.AttnDesc()
+    d.B, d.H, d.Sq, d.D = q.shape
+    d.Hkv, d.Skv = k.shape[1:3]
+    d.dtype = capi.KCG_BF16
+    d.causal = 1 if causal else 0
+    d.scale = float(scale)
+    d.q, d.k, d.v = _strides(q), _strides(k), _strides(v)
+    return d
+
+
+def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float = 1.0, causal: bool = False,
+                  out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`fmha` for a forward pass that will be differentiated: (O, lse), lse[b, h, i] = log sum_j
+    exp(scale q_i.k_j) in float32 [B, H, Sq] (-inf, and O = 0, for a query that sees no key).
+    bfloat16 [B, H, S, D] views with any strides that are multiples of 16 bytes and stride 1 in the
+    last dimension (heads of a packed projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may
+    have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.
+    O is contiguous unless `out` is given."""
+    dev = _require_cuda(q, k, v)
+    d = _attn_desc(q, k, v, scale, causal)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _check_heads("out", out, q.shape, q.dtype, dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
+    d.o = _strides(out)
+    with torch.cuda.device(dev):
+        st = capi.load().kcg_fmha_fwd_lse_launch(ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                                 lse.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    capi.check(st, "kcg_fmha_fwd_lse_launch")
+    return out, lse
+
+
+def fmha_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                  lse: torch.Tensor, *, scale: float = 1.0, causal: bool = False, dq: Optional[torch.Tensor] = None,
+                  dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dQ, dK, dV) of `fmha_with_lse`, from the gradient of its O and the `out` and `lse` it returned
+    (call with the same scale and causal).  Views as there; the gradients are contiguous unless dq, dk or
+    dv is given, e.g. as the heads of a packed gradient.  Outputs must not overlap one another or an
+    input.  The same bits on every call: nothing is added up in an order that can change."""
+    dev = _require_cuda(dout, q, k, v, out, lse)
+    d = _attn_desc(q, k, v, scale, causal)
+    _check_heads("dout", dout, q.shape, q.dtype, dev)
+    _check_heads("out", out, q.shape, q.dtype, dev)
+    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be the contiguous float32 [B,H,Sq] tensor of fmha_with_lse")
+    grads = []
+    for name, g, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if g is None:
+            g = torch.empty(like.shape, dtype=like.dtype, device=dev)
+        else:
+            _check_heads(name, g, like.shape, like.dtype, dev)
+        grads.append(g)
+    dq, dk, dv = grads
+    d.o, d.d_o, d.d_q, d.d_k, d.d_v = (_strides(t) for t in (out, dout, dq, dk, dv))
+    lib = capi.load()
+    with torch.cuda.device(dev):
+        # a buffer of this call alone, from the stream's allocator: two captured graphs never share it
+        ws_bytes = lib.kcg_fmha_bwd_workspace_bytes(ctypes.byref(d))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        st = lib.kcg_fmha_bwd_launch(ctypes.byref(d), dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                     out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                     ws.data_ptr(), ws_bytes, torch.cuda.current_stream(dev).cuda_stream)
+    capi.check(st, "kcg_fmha_bwd_launch")
+    return dq, dk, dv
+
+
+def _rope_desc(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
+    """Checks what both directions of qk_norm_rope take and fills the descriptor's shared part."""
+    dev = q.device
+    if q.dim() != 4:
+        raise ValueError("expected queries (and keys) as [B, heads, S, D]")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {q.dtype}: the kernels take float32 or bfloat16")
+    B, H, S, D = q.shape
+    _check_heads("q", q, q.shape, q.dtype, dev)
+    if k is not None:
+        if k.dim() != 4:
+            raise ValueError("expected queries (and keys) as [B, heads, S, D]")
+        _check_heads("k", k, (B, k.shape[1], S, D), q.dtype, dev)
+    elif k_weight is not None:
+        raise ValueError("k_weight without keys")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise ValueError("cos and sin must be [positions, R / 2] with R <= D")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.float32 or not t.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous float32 table")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if w.shape != (D,) or not w.is_contiguous() or w.dtype != weights[0].dtype or w.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("the weights must be contiguous [D] tensors, both float32 or both bfloat16")
+    d = capi.RopeDesc()
+    d.B, d.S, d.H, d.Hk, d.D, d.R = B, S, H, k.shape[1] if k is not None else 0, D, 2 * cos.shape[1]
+    d.dtype = _dtype_code(q.dtype)
+    d.dtype_w = _dtype_code(weights[0].dtype) if weights else capi.KCG_F32
+    d.interleaved = 1 if interleaved else 0
+    d.table_rows = cos.shape[0]
+    d.eps = float(eps)
+    d.pos_bits = 32
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError("positions must be int32 or int64")
+        if tuple(positions.shape) not in ((S,), (B, S)):
+            raise ValueError(f"positions must be [{S}] or [{B}, {S}]")
+        d.pos_bits = 64 if positions.dtype == torch.int64 else 32
+        d.pos = (ctypes.c_int64 * 2)(positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
+    elif S > cos.shape[0]:
+        raise ValueError("more tokens than rows of the tables")
+    _require_cuda(*[t for t in (q, k, cos, sin, *weights, positions) if t is not None])
+    d.q = _strides(q)
+    if k is not None:
+        d.k = _strides(k)
+    return d
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _like(name: str, given: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    if given is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    _check_heads(name, given, like.shape, like.dtype, like.device)
+    return given
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, *,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None
+                 ) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """What attention wants done to queries and keys first, in one pass: every head row x becomes
+    x / sqrt(mean(x^2) + eps) * weight (weight [D], ones when None), and the pairs (a, b) of its first
+    R entries are rotated to (a cos - b sin, b cos + a sin).  q is a [B, H, S, D] view, k a [B, Hk, S, D]
+    one or None, float32 or bfloat16, any strides but 1 in the last dimension; D even, at most 256.
+    cos, sin: float32 [positions, R / 2] tables; pairs are (i, i + R/2), or (2i, 2i + 1) if `interleaved`.
+    positions: int32 or int64 [S] or [B, S], None for 0..S-1; a position outside the tables makes the
+    row's rotated entries NaN and sets `last_device_status()` to 11.
+    The outputs are contiguous [B, heads, S, D] unless q_out / k_out is given (a slice of a key cache, or
+    the input itself)."""
+    d = _rope_desc(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
+    q_out = _like("q_out", q_out, q)
+    d.q_out = _strides(q_out)
+    if k is not None:
+        k_out = _like("k_out", k_out, k)
+        d.k_out = _strides(k_out)
+    elif k_out is not None:
+        raise ValueError("k_out without keys")
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return q_out, k_out
+    dev = q.device
+    with torch.cuda.device(dev):
+        st = capi.load().kcg_qk_norm_rope_launch(ctypes.byref(d), q.data_ptr(), _ptr(k), _ptr(q_weight), _ptr(k_weight),
+                                                 cos.data_ptr(), sin.data_ptr(), _ptr(positions), q_out.data_ptr(),
+                                                 _ptr(k_out), torch.cuda.current_stream(dev).cuda_stream)
+    capi.check(st, "kcg_qk_norm_rope_launch")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor],
+                          cos: torch.Tensor, sin: torch.Tensor, *, q_weight: Optional[torch.Tensor] = None,
+                          k_weight: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                          eps: float = 1e-6, interleaved: bool = False, dq: Optional[torch.Tensor] = None,
+                          dk: Optional[torch.Tensor] = None
+                          ) -> tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dq, dk, dq_weight, dk_weight) of `qk_norm_rope` for the gradients of its outputs and the inputs
+    it was called with.  The weights' gradients are float32 [D], summed over batch, heads and tokens in a
+    fixed order (None for a weight that is None).  dq and dk are contiguous unless given; they may be
+    dq_out and dk_out themselves."""
+    d = _rope_desc(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
+    dev = q.device
+    if (dk_out is None) != (k is None) or (k is None and dk is not None):
+        raise ValueError("keys and their gradients go together")
+    _check_heads("dq_out", dq_out, q.shape, q.dtype, dev)
+    dq = _like("dq", dq, q)
+    d.q_out, d.d_q = _strides(dq_out), _strides(dq)
+    if k is not None:
+        _check_heads("dk_out", dk_out, k.shape, k.dtype, dev)
+        dk = _like("dk", dk, k)
+        d.k_out, d.d_k = _strides(dk_out), _strides(dk)
+    new = torch.zeros if q.numel() == 0 else torch.empty
+    dqw, dkw = (new(q.shape[3], dtype=torch.float32, device=dev) if w is not None else None for w in (q_weight, k_weight))
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return dq, dk, dqw, dkw
+    lib = capi.load()
+    with torch.cuda.device(dev):
+        # a buffer of this call alone, from the stream's allocator: two captured graphs never share it
+        ws_bytes = lib.kcg_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(d)) if dqw is not None or dkw is not None else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        st = lib.kcg_qk_norm_rope_bwd_launch(ctypes.byref(d), dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k),
+                                             _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions),
+                                             dq.data_ptr(), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws), ws_bytes,
+                                             torch.cuda.current_stream(dev).cuda_stream)
+    capi.check(st, "kcg_qk_norm_rope_bwd_launch")
+    return dq, dk, dqw, dkw
+
+
 def softmax(x: torch.Tensor, *, inplace: bool = False) -> torch.Tensor:
     """Last-axis softmax of an fp32 tensor (the reference's standalone Softmax operator)."""
     dev = _require_cuda(x)

@@ -224,3 +224,150 @@ def test_launch_geometry_follows_the_variant_choice(native_lib):
     out4 = (ctypes.c_int32 * 4)()
     assert native_lib.kcg_fmha_launch_geometry(ctypes.byref(f), out4) == capi.KCG_OK
     assert list(out4) == [32 * 256, 384, 256, 128]
+
+
+def _attn_desc(B=1, H=2, Hkv=1, Sq=128, Skv=128, D=64):
+    d = capi.AttnDesc()
+    d.B, d.H, d.Hkv, d.Sq, d.Skv, d.D = B, H, Hkv, Sq, Skv, D
+    d.dtype = capi.KCG_BF16
+    d.scale = 1.0
+    for name, heads, S in (("q", H, Sq), ("k", Hkv, Skv), ("v", Hkv, Skv), ("o", H, Sq), ("d_o", H, Sq), ("d_q", H, Sq),
+                           ("d_k", Hkv, Skv), ("d_v", Hkv, Skv)):
+        setattr(d, name, (ctypes.c_int64 * 3)(heads * S * D, S * D, D))
+    return d
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(H=3, Hkv=2), capi.KCG_BAD_SHAPE), (dict(Hkv=0), capi.KCG_BAD_SHAPE), (dict(Sq=0), capi.KCG_BAD_SHAPE),
+    (dict(Skv=-1), capi.KCG_BAD_SHAPE), (dict(D=96), capi.KCG_BAD_SHAPE), (dict(Sq=2 ** 31 - 1), capi.KCG_BAD_SHAPE),
+    (dict(dtype=capi.KCG_F32), capi.KCG_UNSUPPORTED), (dict(scale=0.0), capi.KCG_BAD_ARGUMENT),
+    (dict(scale=float("nan")), capi.KCG_BAD_ARGUMENT), (dict(scale=float("inf")), capi.KCG_BAD_ARGUMENT),
+])
+def test_attention_training_descriptor_checks(native_lib, change, want):
+    d = _attn_desc()
+    for name, value in change.items():
+        setattr(d, name, value)
+    at = 0x10000   # never dereferenced: validation fails first
+    assert native_lib.kcg_fmha_fwd_lse_launch(ctypes.byref(d), *[at] * 5, None) == want
+    assert native_lib.kcg_fmha_bwd_launch(ctypes.byref(d), *[at] * 10, 1 << 30, None) == want
+    assert native_lib.kcg_fmha_bwd_workspace_bytes(ctypes.byref(d)) == 0
+
+
+def test_attention_training_pointer_and_stride_checks(native_lib):
+    at = 0x10000
+    d = _attn_desc()
+    assert native_lib.kcg_fmha_fwd_lse_launch(None, *[at] * 5, None) == capi.KCG_BAD_ARGUMENT
+    for i in range(5):
+        ptrs = [at] * 5
+        ptrs[i] = None
+        assert native_lib.kcg_fmha_fwd_lse_launch(ctypes.byref(d), *ptrs, None) == capi.KCG_BAD_ARGUMENT
+        ptrs[i] = at + 2
+        assert native_lib.kcg_fmha_fwd_lse_launch(ctypes.byref(d), *ptrs, None) == capi.KCG_BAD_ALIGN
+    for i in range(9):
+        ptrs = [at] * 10
+        ptrs[i] = None
+        assert native_lib.kcg_fmha_bwd_launch(ctypes.byref(d), *ptrs, 1 << 30, None) == capi.KCG_BAD_ARGUMENT
+        ptrs[i] = at + 2
+        assert native_lib.kcg_fmha_bwd_launch(ctypes.byref(d), *ptrs, 1 << 30, None) == capi.KCG_BAD_ALIGN
+    need = native_lib.kcg_fmha_bwd_workspace_bytes(ctypes.byref(d))
+    assert need >= 2 * 2 * 128 * 4
+    for ws, size in ((None, need), (at, need - 1), (at + 4, need)):
+        assert native_lib.kcg_fmha_bwd_launch(ctypes.byref(d), *[at] * 9, ws, size, None) == capi.KCG_BAD_WORKSPACE
+    for name, calls in (("k", 2), ("v", 2), ("o", 2), ("d_k", 1)):
+        for axis, stride, want in ((2, 68, capi.KCG_BAD_ALIGN), (2, 0, capi.KCG_BAD_SHAPE), (2, -64, capi.KCG_BAD_SHAPE),
+                                   (2, 1 << 40, capi.KCG_BAD_SHAPE)):
+            d = _attn_desc()
+            getattr(d, name)[axis] = stride
+            if calls == 2:
+                assert native_lib.kcg_fmha_fwd_lse_launch(ctypes.byref(d), *[at] * 5, None) == want
+            assert native_lib.kcg_fmha_bwd_launch(ctypes.byref(d), *[at] * 10, 1 << 30, None) == want
+
+
+def _rope_desc(B=1, S=16, H=2, Hk=1, D=64, R=64, dt=capi.KCG_F32):
+    d = capi.RopeDesc()
+    d.B, d.S, d.H, d.Hk, d.D, d.R = B, S, H, Hk, D, R
+    d.dtype = d.dtype_w = dt
+    d.pos_bits, d.table_rows, d.eps = 32, 16, 1e-6
+    for name, heads in (("q", H), ("k", Hk), ("q_out", H), ("k_out", Hk), ("d_q", H), ("d_k", Hk)):
+        setattr(d, name, (ctypes.c_int64 * 3)(heads * S * D, S * D, D))
+    return d
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(B=0), capi.KCG_BAD_SHAPE), (dict(S=0), capi.KCG_BAD_SHAPE), (dict(H=0), capi.KCG_BAD_SHAPE), (dict(Hk=-1), capi.KCG_BAD_SHAPE),
+    (dict(D=63), capi.KCG_BAD_SHAPE), (dict(D=258, R=2), capi.KCG_BAD_SHAPE), (dict(R=0), capi.KCG_BAD_SHAPE),
+    (dict(R=66), capi.KCG_BAD_SHAPE), (dict(R=31), capi.KCG_BAD_SHAPE), (dict(table_rows=0), capi.KCG_BAD_SHAPE),
+    (dict(dtype=2), capi.KCG_UNSUPPORTED), (dict(dtype_w=7), capi.KCG_UNSUPPORTED), (dict(pos_bits=16), capi.KCG_UNSUPPORTED),
+    (dict(eps=-1.0), capi.KCG_BAD_ARGUMENT), (dict(eps=float("nan")), capi.KCG_BAD_ARGUMENT),
+])
+def test_norm_rotation_descriptor_checks(native_lib, change, want):
+    d = _rope_desc()
+    for name, value in change.items():
+        setattr(d, name, value)
+    at = 0x10000
+    assert native_lib.kcg_qk_norm_rope_launch(ctypes.byref(d), *[at] * 9, None) == want
+    assert native_lib.kcg_qk_norm_rope_bwd_launch(ctypes.byref(d), *[at] * 14, 1 << 30, None) == want
+    assert native_lib.kcg_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(d)) == 0
+
+
+def test_norm_rotation_pointer_and_stride_checks(native_lib):
+    at = 0x10000
+    d = _rope_desc()
+    assert native_lib.kcg_qk_norm_rope_launch(None, *[at] * 9, None) == capi.KCG_BAD_ARGUMENT
+    for i in (0, 1, 4, 5, 7, 8):                     # q, k, cos, sin, q_out, k_out
+        ptrs = [at] * 9
+        ptrs[i] = None
+        assert native_lib.kcg_qk_norm_rope_launch(ctypes.byref(d), *ptrs, None) == capi.KCG_BAD_ARGUMENT
+    for i in range(9):
+        ptrs = [at] * 9
+        ptrs[i] = at + 2
+        assert native_lib.kcg_qk_norm_rope_launch(ctypes.byref(d), *ptrs, None) == capi.KCG_BAD_ALIGN
+    for i in (0, 1, 2, 3, 6, 7, 9, 10):              # the gradients, q, k, cos, sin, dq, dk
+        ptrs = [at] * 14
+        ptrs[i] = None
+        assert native_lib.kcg_qk_norm_rope_bwd_launch(ctypes.byref(d), *ptrs, 1 << 30, None) == capi.KCG_BAD_ARGUMENT
+    for name in ("q_out", "k_out"):
+        d = _rope_desc()
+        getattr(d, name)[2] = 0
+        assert native_lib.kcg_qk_norm_rope_launch(ctypes.byref(d), *[at] * 9, None) == capi.KCG_BAD_SHAPE
+    for name in ("d_q", "d_k", "q"):
+        d = _rope_desc()
+        getattr(d, name)[2] = -64
+        assert native_lib.kcg_qk_norm_rope_bwd_launch(ctypes.byref(d), *[at] * 14, 1 << 30, None) == capi.KCG_BAD_SHAPE
+
+
+def test_training_struct_layouts_match_header(tmp_path):
+    import subprocess
+
+    lines = []
+    for cname, cls in (("kcg_attn_desc", capi.AttnDesc), ("kcg_rope_desc", capi.RopeDesc)):
+        lines.append(f'printf("%zu\\n", sizeof({cname}));')
+        lines += [f'printf("%zu\\n", offsetof({cname}, {fname}));' for fname, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "kcg_capi.h"\nint main(void) {\n'
+                   + "\n".join(lines) + "\nreturn 0; }\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for cls in (capi.AttnDesc, capi.RopeDesc):
+        want += [ctypes.sizeof(cls)] + [getattr(cls, fname).offset for fname, _ in cls._fields_]
+    assert got == want
+
+
+def test_training_operators_refuse_cpu_tensors(native_lib):
+    import torch
+
+    from kernelcodegen_b200 import ops
+
+    z = torch.zeros(1, 1, 128, 64, dtype=torch.bfloat16)
+    lse = torch.zeros(1, 1, 128)
+    table = torch.zeros(128, 32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.fmha_with_lse(z, z, z)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.fmha_backward(z, z, z, z, z, lse)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.qk_norm_rope(z, z, table, table)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.qk_norm_rope_backward(z, z, z, z, table, table)

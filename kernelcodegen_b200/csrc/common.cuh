@@ -59,6 +59,19 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
     }                                                                             \
   } while (0)
 
+// Allows a kernel its dynamic shared memory, once per device (the call costs about a microsecond of a
+// launch).  `done`: one flag per device, owned by the caller, one set for each kernel.
+template <typename K>
+kcg_status_t allow_smem(K kern, int bytes, std::atomic<bool> (&done)[64]) {
+  int dev = 0;
+  KCG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return KCG_UNSUPPORTED;
+  if (done[dev].load(std::memory_order_acquire)) return KCG_OK;
+  KCG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done[dev].store(true, std::memory_order_release);
+  return KCG_OK;
+}
+
 kcg_status_t gemm_launch_impl(const kcg_gemm_desc* d, const void* A, const void* B, void* C,
                               void* ws, size_t ws_bytes, cudaStream_t stream);
 size_t gemm_workspace_impl(const kcg_gemm_desc* d);

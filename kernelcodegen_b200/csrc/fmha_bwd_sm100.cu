@@ -94,6 +94,21 @@ struct BwdSmem {
   uint32_t bar_fixed, bar_xfull, bar_xempty, bar_yfull, bar_yempty, bar_sfull, bar_pfull, bar_dpfull, bar_dsfull, bar_done;
 };
 
+// 2^x of pair k of a row: a share of the pairs (a fixed pattern, so that the two kinds of instruction
+// interleave) takes the FMA-pipe polynomial, the rest the MUFU unit, which alone would need 1024 clocks
+// for a 128 x 128 tile, as long as two of the tile's products.
+constexpr int POLY_EIGHTHS = 3;
+__device__ __forceinline__ float2 exp2_share(int k, float2 x) {
+  if (((k * 5) & 7) < POLY_EIGHTHS) {
+    x.x = fmaxf(x.x, -125.f);   // the polynomial's lower end: such a P is 2^-125, nothing in any sum
+    x.y = fmaxf(x.y, -125.f);
+    return ex2_quartic2(x);
+  }
+  x.x = ex2_approx(x.x);
+  x.y = ex2_approx(x.y);
+  return x;
+}
+
 // Two bf16 rows of 32 columns each from 64 floats: the A operand's form, two elements per TMEM column.
 __device__ __forceinline__ void store_a_half(uint32_t taddr, const float2 (&v)[32]) {
   uint32_t pk[32];
@@ -330,21 +345,18 @@ __device__ __forceinline__ void bwd_item(const CUtensorMap* tmA0, const CUtensor
       if (!ok) break;
       tc_fence_after();
       float2 pv[32];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t sr[32];
-        tmem_ld_32x32(s_addr + 32 * g, sr);
+      {
+        uint32_t sr[2][32];
+        tmem_ld_32x32(s_addr, sr[0]);
+        tmem_ld_32x32(s_addr + 32, sr[1]);
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
+        for (int k = 0; k < 32; k += 2) {
           float4 l4 = make_float4(nl, nl, nl, nl);
-          if (KV) l4 = *reinterpret_cast<const float4*>(nl_s + 32 * g + 2 * k);
-          float2 x0 = fma2(make_float2(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1])), make_float2(c, c),
-                           make_float2(l4.x, l4.y));
-          float2 x1 = fma2(make_float2(__uint_as_float(sr[2 * k + 2]), __uint_as_float(sr[2 * k + 3])), make_float2(c, c),
-                           make_float2(l4.z, l4.w));
-          pv[16 * g + k] = make_float2(ex2_approx(x0.x), ex2_approx(x0.y));
-          pv[16 * g + k + 1] = make_float2(ex2_approx(x1.x), ex2_approx(x1.y));
+          if (KV) l4 = *reinterpret_cast<const float4*>(nl_s + 2 * k);
+          const uint32_t* f = &sr[k >> 4][2 * (k & 15)];
+          pv[k] = exp2_share(k, fma2(make_float2(__uint_as_float(f[0]), __uint_as_float(f[1])), make_float2(c, c), make_float2(l4.x, l4.y)));
+          pv[k + 1] = exp2_share(k + 1, fma2(make_float2(__uint_as_float(f[2]), __uint_as_float(f[3])), make_float2(c, c), make_float2(l4.z, l4.w)));
         }
       }
       if (mask) {
@@ -363,19 +375,18 @@ __device__ __forceinline__ void bwd_item(const CUtensorMap* tmA0, const CUtensor
       ok = mbar_wait(sm.bar_dpfull, i & 1u, abort_flag, p.status, DEV_TIMEOUT_PV, p.spin);
       if (!ok) break;
       tc_fence_after();
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t dr[32];
-        tmem_ld_32x32(t_col + TM_DP + 32 * g, dr);
+      {
+        uint32_t dr[2][32];
+        tmem_ld_32x32(t_col + TM_DP, dr[0]);
+        tmem_ld_32x32(t_col + TM_DP + 32, dr[1]);
         tmem_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
+        for (int k = 0; k < 32; k += 2) {
           float4 d4 = make_float4(nd, nd, nd, nd);
-          if (KV) d4 = *reinterpret_cast<const float4*>(nl_s + BT + 32 * g + 2 * k);
-          const float2 e0 = add2(make_float2(__uint_as_float(dr[2 * k]), __uint_as_float(dr[2 * k + 1])), make_float2(d4.x, d4.y));
-          const float2 e1 = add2(make_float2(__uint_as_float(dr[2 * k + 2]), __uint_as_float(dr[2 * k + 3])), make_float2(d4.z, d4.w));
-          pv[16 * g + k] = mul2(pv[16 * g + k], e0);
-          pv[16 * g + k + 1] = mul2(pv[16 * g + k + 1], e1);
+          if (KV) d4 = *reinterpret_cast<const float4*>(nl_s + BT + 2 * k);
+          const uint32_t* f = &dr[k >> 4][2 * (k & 15)];
+          pv[k] = mul2(pv[k], add2(make_float2(__uint_as_float(f[0]), __uint_as_float(f[1])), make_float2(d4.x, d4.y)));
+          pv[k + 1] = mul2(pv[k + 1], add2(make_float2(__uint_as_float(f[2]), __uint_as_float(f[3])), make_float2(d4.z, d4.w)));
         }
       }
       store_a_half(t_col + TM_DP, pv);
@@ -564,7 +575,9 @@ kcg_status_t launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   using Cfg = BwdCfg<D>;
   static_assert(Cfg::SMEM_TOTAL <= 232448, "shared memory budget");
   auto kern = fmha_bwd_kernel<D>;
-  KCG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_TOTAL));
+  static std::atomic<bool> allowed[64];
+  const kcg_status_t st = allow_smem(kern, Cfg::SMEM_TOTAL, allowed);
+  if (st != KCG_OK) return st;
   const long long want = (s.rows * (D / 8) + 255) / 256, most = 8ll * device_sm_count();
   fmha_bwd_stat_kernel<D><<<static_cast<unsigned>(want < most ? want : most), 256, 0, stream>>>(s);
   g_launches.fetch_add(1);

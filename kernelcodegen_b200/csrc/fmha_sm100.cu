@@ -595,8 +595,9 @@ kcg_status_t launch_fmha(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   using Cfg = FmhaCfg<D, TF>;
   static_assert(Cfg::SMEM_TOTAL <= 232448, "shared memory budget");
   auto kern = fmha_fwd_kernel<D, TF, LSE>;
-  KCG_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Cfg::SMEM_TOTAL));
+  static std::atomic<bool> allowed[64];
+  const kcg_status_t st = allow_smem(kern, Cfg::SMEM_TOTAL, allowed);
+  if (st != KCG_OK) return st;
   FmhaParams pp = p;
   pp.after_cast = after_cast ? 1 : 0;
   pp.n_qp = (p.Sq + QTILES * BQ - 1) / (QTILES * BQ);

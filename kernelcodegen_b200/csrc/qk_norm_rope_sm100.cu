@@ -10,13 +10,13 @@
 // Memory-bound: every row is read once and written once (backward: x and dy read, dx written).  All
 // sums are fp32; the results are rounded once, to the type of the tensors.
 //
-// A row belongs to a group of lanes of one warp.  In the vector path a lane holds two 16-byte vectors
-// of the row, chosen so that both members of each of its pairs are its own (vectors j and j + R/2
-// entries; any two when the pairs are neighbours), so the rotation needs no exchange, and the row sums
-// are one shuffle tree.  The group walks several heads of ONE token with the lane's angles and weights
-// in registers: read per row, the tables would be as much traffic as the row itself.  Rows whose size,
-// alignment or R does not split that way take a second kernel, one row at a time, that
-// exchanges the pairs through shared memory.
+// A row belongs to a group of lanes of one warp, and a lane holds both members of each of its pairs, so
+// the rotation needs no exchange and the row sums are one shuffle tree.  The group walks several heads
+// of ONE token with the lane's angles and weights in registers: fetched per row they would be as much
+// traffic as the row itself.  Two forms:
+//   vectors  two 16-byte vectors of the row per lane (vectors j and j + R/2 entries; neighbouring ones
+//            when the pairs are neighbours): D a multiple of a vector, R of two (of one), 16-byte rows
+//   pairs    every other shape and alignment: single entries, consecutive pairs in consecutive lanes
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -40,9 +40,9 @@ struct RopeParams {
   long long pos_sb, pos_ss;
   int B, S, D, R, heads[2];
   int interleaved;
-  float eps;
+  float eps, inv_d;
   int chunk[2], chunks[2];        // heads a group walks; how many such runs a token has
-  long long units[2];             // B * S * chunks
+  unsigned units[2];              // B * S * chunks
   int ctas[2];                    // backward: CTAs of each tensor
   float* part;                    // backward: [ctas][D] partial weight gradients; null when none is wanted
   int* status;
@@ -55,16 +55,14 @@ struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  __device__ static void unpack(const uint4 v, float (&f)[8]) {
+  __device__ static void unpack(const uint4 v, float2 (&f)[4]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
   }
-  __device__ static uint4 pack(const float (&f)[8]) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  __device__ static uint4 pack(const float2 (&f)[4]) {
+    return make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                      pack_bf16x2(f[3].x, f[3].y));
   }
   __device__ static float one(const __nv_bfloat16 v) { return __bfloat162float(v); }
   __device__ static __nv_bfloat16 round(float v) { return __float2bfloat16(v); }
@@ -72,20 +70,45 @@ struct Vec<__nv_bfloat16> {
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  __device__ static void unpack(const uint4 v, float (&f)[4]) {
-    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  __device__ static void unpack(const uint4 v, float2 (&f)[2]) {
+    f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  __device__ static uint4 pack(const float (&f)[4]) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  __device__ static uint4 pack(const float2 (&f)[2]) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
   }
   __device__ static float one(const float v) { return v; }
   __device__ static float round(float v) { return v; }
 };
 
-__device__ __forceinline__ float weight_at(const RopeParams& p, int which, int i) {
-  if (!p.w[which]) return 1.f;
-  return p.w_f32 ? static_cast<const float*>(p.w[which])[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.w[which])[i]);
+// Both weights as fp32 in shared memory, ones where there is none.
+__device__ __forceinline__ void stage_weights(const RopeParams& p, float (&w)[2][256]) {
+  for (int i = threadIdx.x; i < 2 * p.D; i += RN_THREADS) {
+    const int t = i >= p.D, k = i - t * p.D;
+    float v = 1.f;
+    if (p.w[t]) v = p.w_f32 ? static_cast<const float*>(p.w[t])[k] : __bfloat162float(static_cast<const __nv_bfloat16*>(p.w[t])[k]);
+    w[t][k] = v;
+  }
 }
+
+// A group's work: some heads of one token of one of the tensors.
+struct Unit {
+  int type, b, s, h_first, n_heads;
+  // every group of a warp takes part in its rounds (shuffles inside); one past the end has no heads
+  __device__ Unit(const RopeParams& p, unsigned u, bool live, int fixed_type) {
+    type = fixed_type;
+    if (type < 0) {
+      type = u >= p.units[0] ? 1 : 0;
+      if (type) u -= p.units[0];
+    }
+    const unsigned chunks = p.chunks[type], token = u / chunks;
+    h_first = static_cast<int>(u - token * chunks) * p.chunk[type];
+    b = static_cast<int>(token / p.S);
+    s = static_cast<int>(token - static_cast<unsigned>(b) * p.S);
+    n_heads = live ? min(p.chunk[type], p.heads[type] - h_first) : 0;
+  }
+  __device__ long long offset(const long long (&st)[3]) const { return b * st[0] + h_first * st[1] + s * st[2]; }
+};
 
 // Row of the tables for token (b, s), or -1: a position outside the tables is recorded in the status
 // word, and its rotated entries come out as NaN.
@@ -107,15 +130,21 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// Vector path: LPR lanes per row, two vectors per lane.  BWD: the gradients.  U rows are in flight.
-template <typename T, int LPR, bool IL, bool BWD>
-__global__ void __launch_bounds__(RN_THREADS) rope_vec_kernel(const RopeParams p) {
-  constexpr int N = Vec<T>::N;
-  constexpr int GROUPS = RN_THREADS / LPR;
-  constexpr int U = BWD ? 2 : 4;
+__device__ __forceinline__ float2 swap2(float2 v) { return make_float2(v.y, v.x); }
+
+// The vector form: LPR lanes per row, two vectors per lane, U rows in flight
+// while U are computed.  The arithmetic is in pairs
+// of entries (packed fp32), the angles and weights multiplied into the lane's constants once per token:
+//   y_a = r (a * ca + mate_a * sa), with the mate of a vector's entries in the lane's other vector, or
+//   (neighbours) the other entry of the pair.
+template <typename T, int LPR, bool IL, bool BWD, int U>
+__global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_constant__ RopeParams p) {
+  constexpr int N = Vec<T>::N, P = N / 2;
+  constexpr unsigned GROUPS = RN_THREADS / LPR;
+  __shared__ __align__(16) float weights[2][256];
   __shared__ float red[BWD ? RN_THREADS / 32 : 1][BWD ? 256 : 1];
   const int gl = threadIdx.x % LPR;
-  const int group = threadIdx.x / LPR;
+  const unsigned group = threadIdx.x / LPR;
   const int nv = p.D / N;
   // the lane's vectors
   const int hp = IL ? 0 : p.R / (2 * N);
@@ -124,165 +153,177 @@ __global__ void __launch_bounds__(RN_THREADS) rope_vec_kernel(const RopeParams p
   const int vb = mates ? gl + hp : va + 1;
   const bool has_a = va < nv, has_b = vb < nv;
   // whether the lane's vectors are rotated (R is a multiple of a vector)
-  const bool rot_a = IL ? va * N < p.R : mates, rot_b = IL ? vb * N < p.R : mates;
-  float acc_a[N], acc_b[N];
+  const bool rot_a = has_a && (IL ? va * N < p.R : mates), rot_b = has_b && (IL ? vb * N < p.R : mates);
+  float2 acc_a[P], acc_b[P];
   if (BWD) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc_a[i] = acc_b[i] = 0.f;
+    for (int i = 0; i < P; ++i) acc_a[i] = acc_b[i] = make_float2(0.f, 0.f);
   }
-  const long long total = BWD ? 0 : p.units[0] + p.units[1];
-  const int cta_type = BWD && static_cast<int>(blockIdx.x) >= p.ctas[0] ? 1 : 0;
-  const long long end = BWD ? p.units[cta_type] : total;
-  const long long cta = BWD ? static_cast<long long>(blockIdx.x) - (cta_type ? p.ctas[0] : 0) : blockIdx.x;
-  const long long step = static_cast<long long>(BWD ? p.ctas[cta_type] : gridDim.x) * GROUPS;
-  // the same for every lane of the warp, whichever tensor its group is at: there are shuffles inside
+  const int cta_type = BWD ? (static_cast<int>(blockIdx.x) >= p.ctas[0] ? 1 : 0) : -1;
+  const unsigned end = BWD ? p.units[cta_type] : p.units[0] + p.units[1];
+  const unsigned cta = blockIdx.x - (BWD && cta_type ? p.ctas[0] : 0);
+  const unsigned step = (BWD ? p.ctas[cta_type] : gridDim.x) * GROUPS;
   const int rounds = BWD ? p.chunk[cta_type] : max(p.chunk[0], p.chunk[1]);
-  int loaded_type = -1;
-  float wa[N], wb[N];
-  // every lane of a warp makes the same number of rounds (shuffles inside); units past the end idle
-  for (long long u0 = cta * GROUPS; u0 < end; u0 += step) {
-    const long long uu = u0 + group;
-    const bool live = uu < end;
-    long long u = live ? uu : end - 1;
-    int type = cta_type;
-    if (!BWD && u >= p.units[0]) {
-      type = 1;
-      u -= p.units[0];
-    }
-    const long long token = u / p.chunks[type];
-    const int h_first = static_cast<int>(u - token * p.chunks[type]) * p.chunk[type];
-    const int b = static_cast<int>(token / p.S), s = static_cast<int>(token - static_cast<long long>(b) * p.S);
-    const int h_end = min(h_first + p.chunk[type], p.heads[type]);
-    if (type != loaded_type) {
-      loaded_type = type;
+  unsigned u0 = cta * GROUPS;
+  if (u0 >= end) return;
+  // Where a unit's rows are, and the rows of one round: U heads.
+  struct Where {
+    int type, n_heads;
+    long long tr;
+    const T *x, *dy;
+    long long y0;
+  };
+  auto place = [&](unsigned u) {
+    const bool live = u + group < end;
+    const Unit un(p, live ? u + group : end - 1, live, cta_type);
+    Where w;
+    w.type = un.type;
+    w.n_heads = un.n_heads;
+    w.tr = table_row(p, un.b, un.s);
+    w.x = static_cast<const T*>(p.x[un.type]) + un.offset(p.xs[un.type]);
+    w.dy = BWD ? static_cast<const T*>(p.dy[un.type]) + un.offset(p.ds[un.type]) : nullptr;
+    w.y0 = un.offset(p.ys[un.type]);
+    return w;
+  };
+  uint4 xn[U][2], dn[BWD ? U : 1][2];   // the round that is on its way
+  auto load = [&](const Where& w, int h0) {
+    const long long xh = p.xs[w.type][1], dh = p.ds[w.type][1];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        wa[i] = has_a ? weight_at(p, type, va * N + i) : 0.f;
-        wb[i] = has_b ? weight_at(p, type, vb * N + i) : 0.f;
+    for (int k = 0; k < U; ++k) {
+      const bool on = h0 + k < w.n_heads;
+      xn[k][0] = xn[k][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (on && has_a) xn[k][0] = *reinterpret_cast<const uint4*>(w.x + (h0 + k) * xh + va * N);
+      if (on && has_b) xn[k][1] = *reinterpret_cast<const uint4*>(w.x + (h0 + k) * xh + vb * N);
+      if (BWD) {
+        dn[k][0] = dn[k][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (on && has_a) dn[k][0] = *reinterpret_cast<const uint4*>(w.dy + (h0 + k) * dh + va * N);
+        if (on && has_b) dn[k][1] = *reinterpret_cast<const uint4*>(w.dy + (h0 + k) * dh + vb * N);
       }
     }
-    // angles: half-split, pair i of the lane = (a_i, b_i); neighbours, pairs 0.. of a then those of b
-    float c[N], sn[N];
+  };
+  Where un = place(u0);
+  load(un, 0);
+  stage_weights(p, weights);
+  __syncthreads();
+  for (;;) {
+    const int type = un.type;
+    const long long yh = p.ys[type][1];
+    // the lane's constants; backward: ca, sa hold the angles alone, cb, sb the weights
+    float2 ca[P], sa[P], cb[P], sb[P];
     {
-      const long long tr = table_row(p, b, s);
-      const float* ct = p.cs + tr * (p.R / 2);
-      const float* st = p.sn + tr * (p.R / 2);
+      const long long tr = un.tr;
+      // angle of pair i of the lane: half-split, entry i of a with entry i of b; neighbours, first the P
+      // pairs of a, then those of b.  Either way consecutive entries of the tables.
+      float2 c[P], sn[P];
+      const float* ct = p.cs + tr * (p.R / 2) + va * (IL ? P : N);
+      const float* st = p.sn + tr * (p.R / 2) + va * (IL ? P : N);
       const float bad = __int_as_float(0x7FC00000);
-      if (IL) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const bool rot = i < N / 2 ? rot_a && has_a : rot_b && has_b;
-          const int at = i < N / 2 ? va * (N / 2) + i : vb * (N / 2) + i - N / 2;
-          c[i] = rot ? (tr >= 0 ? ct[at] : bad) : 1.f;
-          sn[i] = rot ? (tr >= 0 ? st[at] : bad) : 0.f;
+      for (int i = 0; i < P; ++i) {
+        const bool rot = IL ? (2 * i < P ? rot_a : rot_b) : mates;
+        c[i] = rot ? make_float2(bad, bad) : make_float2(1.f, 1.f);
+        sn[i] = rot ? make_float2(bad, bad) : make_float2(0.f, 0.f);
+        if (rot && tr >= 0) {
+          c[i] = __ldg(reinterpret_cast<const float2*>(ct) + i);
+          sn[i] = __ldg(reinterpret_cast<const float2*>(st) + i);
         }
-      } else {
+      }
+      float2 wa[P], wb[P];
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          float4 c4 = make_float4(bad, bad, bad, bad), s4 = c4;
-          if (mates && tr >= 0) {
-            c4 = *reinterpret_cast<const float4*>(ct + va * N + i);
-            s4 = *reinterpret_cast<const float4*>(st + va * N + i);
-          }
-          c[i] = c4.x, c[i + 1] = c4.y, c[i + 2] = c4.z, c[i + 3] = c4.w;
-          sn[i] = s4.x, sn[i + 1] = s4.y, sn[i + 2] = s4.z, sn[i + 3] = s4.w;
+      for (int i = 0; i < P; ++i) {
+        wa[i] = wb[i] = make_float2(0.f, 0.f);
+        if (has_a) wa[i] = *reinterpret_cast<const float2*>(&weights[type][va * N + 2 * i]);
+        if (has_b) wb[i] = *reinterpret_cast<const float2*>(&weights[type][vb * N + 2 * i]);
+      }
+      auto at = [](const float2 (&v)[P], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; };
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        if (BWD) {
+          ca[i] = c[i];
+          sa[i] = sn[i];
+          cb[i] = wa[i];
+          sb[i] = wb[i];
+        } else if (IL) {
+          const float c0 = at(c, i), s0 = at(sn, i), c1 = at(c, P + i), s1 = at(sn, P + i);
+          ca[i] = make_float2(c0 * wa[i].x, c0 * wa[i].y);
+          sa[i] = make_float2(-s0 * wa[i].y, s0 * wa[i].x);
+          cb[i] = make_float2(c1 * wb[i].x, c1 * wb[i].y);
+          sb[i] = make_float2(-s1 * wb[i].y, s1 * wb[i].x);
+        } else {
+          ca[i] = mul2(c[i], wa[i]);
+          sa[i] = mul2(make_float2(-sn[i].x, -sn[i].y), wb[i]);
+          cb[i] = mul2(c[i], wb[i]);
+          sb[i] = mul2(sn[i], wa[i]);
         }
       }
     }
-    const T* x = static_cast<const T*>(p.x[type]) + b * p.xs[type][0] + s * p.xs[type][2];
-    const T* dy = BWD ? static_cast<const T*>(p.dy[type]) + b * p.ds[type][0] + s * p.ds[type][2] : nullptr;
-    const long long y0 = b * p.ys[type][0] + s * p.ys[type][2];
+    const bool more = u0 + step < end;
+    Where next = un;
+    if (more) next = place(u0 + step);
     for (int h0 = 0; h0 < rounds; h0 += U) {
       uint4 xv[U][2], dv[BWD ? U : 1][2];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int h = h_first + h0 + k;
-        const bool on = live && h0 + k < p.chunk[type] && h < h_end;
-        xv[k][0] = xv[k][1] = make_uint4(0u, 0u, 0u, 0u);
-        if (BWD) dv[k][0] = dv[k][1] = make_uint4(0u, 0u, 0u, 0u);
-        if (on) {
-          const T* xr = x + h * p.xs[type][1];
-          if (has_a) xv[k][0] = *reinterpret_cast<const uint4*>(xr + va * N);
-          if (has_b) xv[k][1] = *reinterpret_cast<const uint4*>(xr + vb * N);
-          if (BWD) {
-            const T* dr = dy + h * p.ds[type][1];
-            if (has_a) dv[k][0] = *reinterpret_cast<const uint4*>(dr + va * N);
-            if (has_b) dv[k][1] = *reinterpret_cast<const uint4*>(dr + vb * N);
-          }
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          xv[k][j] = xn[k][j];
+          if (BWD) dv[k][j] = dn[k][j];
         }
-      }
+      // the next round, of this token or of the group's next one, is on its way while this is computed
+      if (h0 + U < rounds) load(un, h0 + U);
+      else if (more) load(next, 0);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int h = h_first + h0 + k;
-        const bool on = live && h0 + k < p.chunk[type] && h < h_end;
-        float a[N], bb[N], ss = 0.f;
+        const bool on = h0 + k < un.n_heads;
+        float2 a[P], bb[P], s2 = make_float2(0.f, 0.f);
         Vec<T>::unpack(xv[k][0], a);
         Vec<T>::unpack(xv[k][1], bb);
 #pragma unroll
-        for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(bb[i], bb[i], ss));
-        ss = group_sum<LPR>(ss);
-        const float r = rsqrtf(ss / p.D + p.eps);
-        float oa[N], ob[N];
+        for (int i = 0; i < P; ++i) s2 = fma2(bb[i], bb[i], fma2(a[i], a[i], s2));
+        const float r = rsqrtf(group_sum<LPR>(s2.x + s2.y) * p.inv_d + p.eps);
+        const float2 r2 = make_float2(r, r);
+        float2 oa[P], ob[P];
         if (!BWD) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            oa[i] = a[i] * r * wa[i];
-            ob[i] = bb[i] * r * wb[i];
-          }
-          if (IL) {
-#pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-              const float a0 = oa[2 * i], a1 = oa[2 * i + 1], b0 = ob[2 * i], b1 = ob[2 * i + 1];
-              if (rot_a) oa[2 * i] = a0 * c[i] - a1 * sn[i], oa[2 * i + 1] = a1 * c[i] + a0 * sn[i];
-              if (rot_b) ob[2 * i] = b0 * c[N / 2 + i] - b1 * sn[N / 2 + i], ob[2 * i + 1] = b1 * c[N / 2 + i] + b0 * sn[N / 2 + i];
-            }
-          } else if (mates) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const float f = oa[i], g = ob[i];
-              oa[i] = f * c[i] - g * sn[i];
-              ob[i] = g * c[i] + f * sn[i];
-            }
+          for (int i = 0; i < P; ++i) {
+            oa[i] = mul2(fma2(IL ? swap2(a[i]) : bb[i], sa[i], mul2(a[i], ca[i])), r2);
+            ob[i] = mul2(fma2(IL ? swap2(bb[i]) : a[i], sb[i], mul2(bb[i], cb[i])), r2);
           }
         } else {
-          float ga[N], gb[N], dot = 0.f;
+          float2 ga[P], gb[P], d2 = make_float2(0.f, 0.f);
           Vec<T>::unpack(dv[k][0], ga);
           Vec<T>::unpack(dv[k][1], gb);
-          if (IL) {
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) {
-              const float a0 = ga[2 * i], a1 = ga[2 * i + 1], b0 = gb[2 * i], b1 = gb[2 * i + 1];
-              if (rot_a) ga[2 * i] = a0 * c[i] + a1 * sn[i], ga[2 * i + 1] = a1 * c[i] - a0 * sn[i];
-              if (rot_b) gb[2 * i] = b0 * c[N / 2 + i] + b1 * sn[N / 2 + i], gb[2 * i + 1] = b1 * c[N / 2 + i] - b0 * sn[N / 2 + i];
+          for (int i = 0; i < P; ++i) {
+            const float2 f = ga[i], g = gb[i];
+            if (IL) {
+              // pair i's angle: entry i of the first half of c and sn for a, of the second for b
+              const float cA = i & 1 ? ca[i / 2].y : ca[i / 2].x, sA = i & 1 ? sa[i / 2].y : sa[i / 2].x;
+              const float cB = (P + i) & 1 ? ca[(P + i) / 2].y : ca[(P + i) / 2].x, sB = (P + i) & 1 ? sa[(P + i) / 2].y : sa[(P + i) / 2].x;
+              ga[i] = fma2(make_float2(f.y, -f.x), make_float2(sA, sA), mul2(f, make_float2(cA, cA)));
+              gb[i] = fma2(make_float2(g.y, -g.x), make_float2(sB, sB), mul2(g, make_float2(cB, cB)));
+            } else {
+              ga[i] = fma2(g, sa[i], mul2(f, ca[i]));
+              gb[i] = fma2(make_float2(-f.x, -f.y), sa[i], mul2(g, ca[i]));
             }
-          } else if (mates) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const float f = ga[i], g = gb[i];
-              ga[i] = f * c[i] + g * sn[i];
-              gb[i] = g * c[i] - f * sn[i];
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (on) {
-              acc_a[i] = fmaf(ga[i] * r, a[i], acc_a[i]);
-              acc_b[i] = fmaf(gb[i] * r, bb[i], acc_b[i]);
-            }
-            ga[i] *= wa[i];
-            gb[i] *= wb[i];
-            dot = fmaf(ga[i], a[i], fmaf(gb[i], bb[i], dot));
+            // rows past the run are zeros: they add nothing
+            acc_a[i] = fma2(ga[i], mul2(a[i], r2), acc_a[i]);
+            acc_b[i] = fma2(gb[i], mul2(bb[i], r2), acc_b[i]);
+            ga[i] = mul2(ga[i], cb[i]);
+            gb[i] = mul2(gb[i], sb[i]);
+            d2 = fma2(gb[i], bb[i], fma2(ga[i], a[i], d2));
           }
           // x r^3 mean(g w x): the factors in an order that neither overflows nor vanishes for tiny rows
-          const float m = group_sum<LPR>(dot * r) / p.D;
+          const float m = -group_sum<LPR>((d2.x + d2.y) * r) * p.inv_d;
+          const float2 m2 = make_float2(m, m);
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            oa[i] = r * (ga[i] - (a[i] * r) * m);
-            ob[i] = r * (gb[i] - (bb[i] * r) * m);
+          for (int i = 0; i < P; ++i) {
+            oa[i] = mul2(fma2(mul2(a[i], r2), m2, ga[i]), r2);
+            ob[i] = mul2(fma2(mul2(bb[i], r2), m2, gb[i]), r2);
           }
         }
         if (on) {
-          const long long at = y0 + h * p.ys[type][1];
+          const long long at = un.y0 + (h0 + k) * yh;
           T* yr = static_cast<T*>(p.y[type]) + at;
           if (has_a && bounds_ok((at + va * N) * sizeof(T), 16, p.y_extent[type], p.status, p.bounds_detail))
             *reinterpret_cast<uint4*>(yr + va * N) = Vec<T>::pack(oa);
@@ -291,23 +332,28 @@ __global__ void __launch_bounds__(RN_THREADS) rope_vec_kernel(const RopeParams p
         }
       }
     }
+    if (!more) break;
+    un = next;
+    u0 += step;
   }
   if (BWD && p.part) {
     // lanes of equal place in their group, then the warps, in a fixed order
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < P; ++i) {
 #pragma unroll
       for (int o = LPR; o < 32; o <<= 1) {
-        acc_a[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_a[i], o);
-        acc_b[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_b[i], o);
+        acc_a[i].x += __shfl_xor_sync(0xFFFFFFFFu, acc_a[i].x, o);
+        acc_a[i].y += __shfl_xor_sync(0xFFFFFFFFu, acc_a[i].y, o);
+        acc_b[i].x += __shfl_xor_sync(0xFFFFFFFFu, acc_b[i].x, o);
+        acc_b[i].y += __shfl_xor_sync(0xFFFFFFFFu, acc_b[i].y, o);
       }
     }
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) < LPR) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (has_a) red[warp][va * N + i] = acc_a[i];
-        if (has_b) red[warp][vb * N + i] = acc_b[i];
+      for (int i = 0; i < P; ++i) {
+        if (has_a) red[warp][va * N + 2 * i] = acc_a[i].x, red[warp][va * N + 2 * i + 1] = acc_a[i].y;
+        if (has_b) red[warp][vb * N + 2 * i] = acc_b[i].x, red[warp][vb * N + 2 * i + 1] = acc_b[i].y;
       }
     }
     __syncthreads();
@@ -320,127 +366,145 @@ __global__ void __launch_bounds__(RN_THREADS) rope_vec_kernel(const RopeParams p
   }
 }
 
-// Any even D <= 256, any even R <= D, any alignment: a warp per row; VEC entries per access (16 bytes
-// where the rows allow it), the pairs exchanged through shared memory.
-template <typename T, int VEC, bool BWD>
-__global__ void __launch_bounds__(RN_THREADS) rope_row_kernel(const RopeParams p) {
-  constexpr int WARPS = RN_THREADS / 32;
-  constexpr int PER = 256 / (32 * VEC) ? 256 / (32 * VEC) : 1;   // accesses per lane
-  __shared__ float rows[WARPS][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* row = rows[warp];
-  float acc[PER][VEC];
-#pragma unroll
-  for (int j = 0; j < PER; ++j)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[j][i] = 0.f;
-  const int cta_type = BWD && static_cast<int>(blockIdx.x) >= p.ctas[0] ? 1 : 0;
-  const long long end = BWD ? p.units[cta_type] : p.units[0] + p.units[1];
-  const long long cta = BWD ? static_cast<long long>(blockIdx.x) - (cta_type ? p.ctas[0] : 0) : blockIdx.x;
-  const long long step = static_cast<long long>(BWD ? p.ctas[cta_type] : gridDim.x) * WARPS;
+// The pair form: LPR lanes per row, pairs gl, gl + LPR, .. of the row per lane (first the rotated ones,
+// then the rest of the row two by two), single entries.
+template <typename T, int LPR, int NP, bool BWD, int U>
+__global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_constant__ RopeParams p) {
+  constexpr unsigned GROUPS = RN_THREADS / LPR;
+  __shared__ float weights[2][256];
+  __shared__ float red[BWD ? RN_THREADS / 32 : 1][BWD ? 256 : 1];
+  const int gl = threadIdx.x % LPR;
+  const unsigned group = threadIdx.x / LPR;
   const int half = p.R / 2;
-  // index of entry i's mate, of the pair's angle, and the sign of the mate's term in the forward rotation
-  auto mate = [&](int i) { return p.interleaved ? i ^ 1 : (i < half ? i + half : i - half); };
-  auto angle = [&](int i) { return p.interleaved ? i >> 1 : (i < half ? i : i - half); };
-  auto first = [&](int i) { return p.interleaved ? !(i & 1) : i < half; };
-  for (long long uu = cta * WARPS + warp; uu < end; uu += step) {
-    long long u = uu;
-    int type = cta_type;
-    if (!BWD && u >= p.units[0]) {
-      type = 1;
-      u -= p.units[0];
-    }
-    // a unit is one row here (chunk = 1)
-    const long long token = u / p.heads[type];
-    const int h = static_cast<int>(u - token * p.heads[type]);
-    const int b = static_cast<int>(token / p.S), s = static_cast<int>(token - static_cast<long long>(b) * p.S);
-    const T* x = static_cast<const T*>(p.x[type]) + b * p.xs[type][0] + h * p.xs[type][1] + s * p.xs[type][2];
-    const T* dy = BWD ? static_cast<const T*>(p.dy[type]) + b * p.ds[type][0] + h * p.ds[type][1] + s * p.ds[type][2] : nullptr;
-    const long long y0 = b * p.ys[type][0] + h * p.ys[type][1] + s * p.ys[type][2];
-    T* y = static_cast<T*>(p.y[type]) + y0;
-    float xv[PER][VEC], ss = 0.f;
-    __syncwarp();
+  int ea[NP], eb[NP];    // the pairs' entries; -1: none
+  float acc_a[NP], acc_b[NP];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int at = (j * 32 + lane) * VEC;
-      float other[VEC];
+  for (int i = 0; i < NP; ++i) {
+    const int pr = gl + i * LPR;
+    const bool split = pr < half && !p.interleaved;
+    ea[i] = pr < p.D / 2 ? (split ? pr : 2 * pr) : -1;
+    eb[i] = split ? pr + half : 2 * pr + 1;
+    acc_a[i] = acc_b[i] = 0.f;
+  }
+  stage_weights(p, weights);
+  __syncthreads();
+  const int cta_type = BWD ? (static_cast<int>(blockIdx.x) >= p.ctas[0] ? 1 : 0) : -1;
+  const unsigned end = BWD ? p.units[cta_type] : p.units[0] + p.units[1];
+  const unsigned cta = blockIdx.x - (BWD && cta_type ? p.ctas[0] : 0);
+  const unsigned step = (BWD ? p.ctas[cta_type] : gridDim.x) * GROUPS;
+  const int rounds = BWD ? p.chunk[cta_type] : max(p.chunk[0], p.chunk[1]);
+  for (unsigned u0 = cta * GROUPS; u0 < end; u0 += step) {
+    const bool live = u0 + group < end;
+    const Unit un(p, live ? u0 + group : end - 1, live, cta_type);
+    const int type = un.type;
+    const long long xh = p.xs[type][1], dh = p.ds[type][1], yh = p.ys[type][1];
+    const T* x = static_cast<const T*>(p.x[type]) + un.offset(p.xs[type]);
+    const T* dy = BWD ? static_cast<const T*>(p.dy[type]) + un.offset(p.ds[type]) : nullptr;
+    const long long y0 = un.offset(p.ys[type]);
+    float c[NP], sn[NP], wa[NP], wb[NP];
+    const long long tr = table_row(p, un.b, un.s);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) xv[j][i] = other[i] = 0.f;
-      if (at < p.D) {
-        if constexpr (VEC == 1) {
-          xv[j][0] = Vec<T>::one(x[at]);
-          if (BWD) other[0] = Vec<T>::one(dy[at]);
-        } else {
-          Vec<T>::unpack(*reinterpret_cast<const uint4*>(x + at), xv[j]);
-          if (BWD) Vec<T>::unpack(*reinterpret_cast<const uint4*>(dy + at), other);
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) row[at + i] = BWD ? other[i] : xv[j][i] * weight_at(p, type, at + i);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) ss = fmaf(xv[j][i], xv[j][i], ss);
-    }
-    ss = group_sum<32>(ss);
-    const float r = rsqrtf(ss / p.D + p.eps);
-    const long long tr = table_row(p, b, s);
-    __syncwarp();
-    // forward: y = r * rotation of x w; backward: g = dy rotated back
-    float out[PER][VEC], dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int e = (j * 32 + lane) * VEC + i;
-        out[j][i] = 0.f;
-        if (e >= p.D) continue;
-        float v = row[e];
-        if (e < p.R) {
-          const float c = tr >= 0 ? p.cs[tr * half + angle(e)] : __int_as_float(0x7FC00000);
-          const float sn = tr >= 0 ? p.sn[tr * half + angle(e)] : c;
-          const float m = row[mate(e)] * sn;
-          v = v * c + (first(e) == BWD ? m : -m);
-        }
-        if (BWD) {
-          acc[j][i] = fmaf(v * r, xv[j][i], acc[j][i]);
-          v *= weight_at(p, type, e);
-          dot = fmaf(v, xv[j][i], dot);
-          out[j][i] = v;
-        } else {
-          out[j][i] = r * v;
+    for (int i = 0; i < NP; ++i) {
+      c[i] = 1.f, sn[i] = 0.f, wa[i] = wb[i] = 0.f;
+      const int pr = gl + i * LPR;
+      if (pr < half) {
+        c[i] = sn[i] = __int_as_float(0x7FC00000);
+        if (tr >= 0) {
+          c[i] = __ldg(p.cs + tr * half + pr);
+          sn[i] = __ldg(p.sn + tr * half + pr);
         }
       }
-    if (BWD) {
-      const float m = group_sum<32>(dot * r) / p.D;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) out[j][i] = r * (out[j][i] - (xv[j][i] * r) * m);
+      if (ea[i] >= 0) {
+        wa[i] = weights[type][ea[i]];
+        wb[i] = weights[type][eb[i]];
+      }
     }
+    for (int h0 = 0; h0 < rounds; h0 += U) {
+      float a[U][NP], bb[U][NP], ga[BWD ? U : 1][NP], gb[BWD ? U : 1][NP];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int at = (j * 32 + lane) * VEC;
-      if (at < p.D && bounds_ok((y0 + at) * sizeof(T), VEC * sizeof(T), p.y_extent[type], p.status, p.bounds_detail)) {
-        if constexpr (VEC == 1)
-          y[at] = Vec<T>::round(out[j][0]);
-        else
-          *reinterpret_cast<uint4*>(y + at) = Vec<T>::pack(out[j]);
+      for (int k = 0; k < U; ++k) {
+        const bool on = h0 + k < un.n_heads;
+        const T* xr = x + (h0 + k) * xh;
+        const T* dr = dy + (h0 + k) * dh;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          a[k][i] = bb[k][i] = 0.f;
+          if (BWD) ga[k][i] = gb[k][i] = 0.f;
+          if (on && ea[i] >= 0) {
+            a[k][i] = Vec<T>::one(xr[ea[i]]);
+            bb[k][i] = Vec<T>::one(xr[eb[i]]);
+            if (BWD) {
+              ga[k][i] = Vec<T>::one(dr[ea[i]]);
+              gb[k][i] = Vec<T>::one(dr[eb[i]]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const bool on = h0 + k < un.n_heads;
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(bb[k][i], bb[k][i], ss));
+        const float r = rsqrtf(group_sum<LPR>(ss) * p.inv_d + p.eps);
+        float oa[NP], ob[NP];
+        if (!BWD) {
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const float f = a[k][i] * wa[i], g = bb[k][i] * wb[i];
+            oa[i] = r * (f * c[i] - g * sn[i]);
+            ob[i] = r * (g * c[i] + f * sn[i]);
+          }
+        } else {
+          float dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            const float f = ga[k][i] * c[i] + gb[k][i] * sn[i], g = gb[k][i] * c[i] - ga[k][i] * sn[i];
+            // rows past the run are zeros: they add nothing
+            acc_a[i] = fmaf(f, a[k][i] * r, acc_a[i]);
+            acc_b[i] = fmaf(g, bb[k][i] * r, acc_b[i]);
+            oa[i] = f * wa[i];
+            ob[i] = g * wb[i];
+            dot = fmaf(oa[i], a[k][i], fmaf(ob[i], bb[k][i], dot));
+          }
+          const float m = group_sum<LPR>(dot * r) * p.inv_d;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            oa[i] = r * (oa[i] - (a[k][i] * r) * m);
+            ob[i] = r * (ob[i] - (bb[k][i] * r) * m);
+          }
+        }
+        if (on) {
+          const long long at = y0 + (h0 + k) * yh;
+          T* yr = static_cast<T*>(p.y[type]) + at;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            if (ea[i] < 0) continue;
+            if (bounds_ok((at + ea[i]) * sizeof(T), sizeof(T), p.y_extent[type], p.status, p.bounds_detail)) yr[ea[i]] = Vec<T>::round(oa[i]);
+            if (bounds_ok((at + eb[i]) * sizeof(T), sizeof(T), p.y_extent[type], p.status, p.bounds_detail)) yr[eb[i]] = Vec<T>::round(ob[i]);
+          }
+        }
       }
     }
   }
   if (BWD && p.part) {
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
+    for (int i = 0; i < NP; ++i) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int e = (j * 32 + lane) * VEC + i;
-        if (e < p.D) row[e] = acc[j][i];
+      for (int o = LPR; o < 32; o <<= 1) {
+        acc_a[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_a[i], o);
+        acc_b[i] += __shfl_xor_sync(0xFFFFFFFFu, acc_b[i], o);
       }
+      if ((threadIdx.x & 31) < LPR && ea[i] >= 0) {
+        red[threadIdx.x >> 5][ea[i]] = acc_a[i];
+        red[threadIdx.x >> 5][eb[i]] = acc_b[i];
+      }
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < p.D; i += RN_THREADS) {
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < WARPS; ++k) sum += rows[k][i];
+      for (int k = 0; k < RN_THREADS / 32; ++k) sum += red[k][i];
       p.part[static_cast<long long>(blockIdx.x) * p.D + i] = sum;
     }
   }
@@ -477,27 +541,36 @@ bool row_vectors(const HeadView& v, int es) {
   return true;
 }
 
-// CTAs that the backward pass may use for each tensor: at most four per SM over both, so that the
+// CTAs that the backward pass may use for each tensor: at most two per SM over both (what is resident), so that the
 // partial weight gradients stay few.  A function of the shape alone (the workspace query has no pointers).
 void bwd_ctas(const kcg_rope_desc* d, int& q, int& k) {
-  const int most = 4 * 148;
+  const int most = 2 * 148;
   const long long heads = static_cast<long long>(d->H) + d->Hk;
   k = d->Hk ? static_cast<int>(most * static_cast<long long>(d->Hk) / heads) : 0;
   if (d->Hk && k < 1) k = 1;
   q = most - k;
 }
 
-template <typename T, int LPR, bool IL, bool BWD>
-void go_vec(const RopeParams& p, unsigned grid, cudaStream_t stream) {
-  rope_vec_kernel<T, LPR, IL, BWD><<<grid, RN_THREADS, 0, stream>>>(p);
-}
 template <typename T, bool IL, bool BWD>
 void go_vec(const RopeParams& p, int lpr, unsigned grid, cudaStream_t stream) {
+  constexpr int U = BWD ? 1 : 2;
   switch (lpr) {
-    case 4: return go_vec<T, 4, IL, BWD>(p, grid, stream);
-    case 8: return go_vec<T, 8, IL, BWD>(p, grid, stream);
-    case 16: return go_vec<T, 16, IL, BWD>(p, grid, stream);
-    default: return go_vec<T, 32, IL, BWD>(p, grid, stream);
+    case 4: return rope_vec_kernel<T, 4, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 8: return rope_vec_kernel<T, 8, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 16: return rope_vec_kernel<T, 16, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    default: return rope_vec_kernel<T, 32, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+  }
+}
+template <typename T, bool BWD>
+void go_pair(const RopeParams& p, unsigned grid, cudaStream_t stream) {
+  constexpr int U = 2;
+  switch ((p.D + 31) / 32) {   // lanes per row x pairs per lane >= D / 2
+    case 1: return rope_pair_kernel<T, 16, 1, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 2: return rope_pair_kernel<T, 16, 2, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 3: return rope_pair_kernel<T, 16, 3, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 4: return rope_pair_kernel<T, 16, 4, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 5: case 6: return rope_pair_kernel<T, 32, 3, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    default: return rope_pair_kernel<T, 32, 4, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
   }
 }
 
@@ -505,41 +578,37 @@ template <typename T, bool BWD>
 kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cudaStream_t stream) {
   constexpr int N = Vec<T>::N;
   const int nv = d->D / N;
-  // the vector path: whole vectors, and both members of each pair in vectors of one lane
+  // the vector form: whole vectors, and both members of each pair in vectors of one lane
   const bool vec = vectors && d->D % N == 0 && (d->interleaved ? d->R % N == 0 : d->R % (2 * N) == 0);
   int lpr = 4;
   while (2 * lpr < nv) lpr *= 2;
-  const int per_cta = vec ? RN_THREADS / lpr : RN_THREADS / 32;
+  const int per_cta = RN_THREADS / (vec ? lpr : d->D <= 128 ? 16 : 32);
   const long long tokens = static_cast<long long>(d->B) * d->S, sms = device_sm_count();
   for (int t = 0; t < 2; ++t) {
     // heads a group walks with one set of angles: as many as leave two groups' worth of work for
-    // every group that the SMs hold (2048 threads each), at most 8
+    // every group that the SMs hold, at most 8
     int chunk = 1;
-    if (vec)
-      while (chunk < 8 && 2 * chunk <= p.heads[t] && tokens * p.heads[t] / (2 * chunk) >= sms * (2048 / RN_THREADS) * per_cta) chunk *= 2;
+    while (chunk < 8 && 2 * chunk <= p.heads[t] && tokens * p.heads[t] / (2 * chunk) >= sms * 8 * per_cta) chunk *= 2;
+    const int chunks = p.heads[t] ? (p.heads[t] + chunk - 1) / chunk : 0;
+    if (tokens * chunks > 0x3FFFFFFFll) return KCG_BAD_SHAPE;
     p.chunk[t] = chunk;
-    p.chunks[t] = p.heads[t] ? (p.heads[t] + chunk - 1) / chunk : 0;
-    p.units[t] = tokens * p.chunks[t];
+    p.chunks[t] = chunks;
+    p.units[t] = static_cast<unsigned>(tokens * chunks);
   }
   unsigned grid;
   if (BWD) {
     for (int t = 0; t < 2; ++t) {
-      const long long want = (p.units[t] + per_cta - 1) / per_cta;
-      if (p.ctas[t] > want) p.ctas[t] = static_cast<int>(want);
+      const unsigned want = (p.units[t] + per_cta - 1) / per_cta;
+      if (static_cast<unsigned>(p.ctas[t]) > want) p.ctas[t] = static_cast<int>(want);
     }
     grid = static_cast<unsigned>(p.ctas[0] + p.ctas[1]);
   } else {
-    const long long want = (p.units[0] + p.units[1] + per_cta - 1) / per_cta, most = 16 * sms;
+    const long long want = (static_cast<long long>(p.units[0]) + p.units[1] + per_cta - 1) / per_cta, most = (vec ? 2 : 16) * sms;
     grid = static_cast<unsigned>(want < most ? want : most);
   }
-  if (vec) {
-    if (d->interleaved) go_vec<T, true, BWD>(p, lpr, grid, stream);
-    else go_vec<T, false, BWD>(p, lpr, grid, stream);
-  } else if (vectors && d->D % N == 0) {
-    rope_row_kernel<T, N, BWD><<<grid, RN_THREADS, 0, stream>>>(p);
-  } else {
-    rope_row_kernel<T, 1, BWD><<<grid, RN_THREADS, 0, stream>>>(p);
-  }
+  if (!vec) go_pair<T, BWD>(p, grid, stream);
+  else if (d->interleaved) go_vec<T, true, BWD>(p, lpr, grid, stream);
+  else go_vec<T, false, BWD>(p, lpr, grid, stream);
   g_launches.fetch_add(1);
   KCG_CUDA_TRY(cudaGetLastError());
   return KCG_OK;
@@ -602,6 +671,7 @@ kcg_status_t fill(const kcg_rope_desc* d, const void* const (&x)[2], const int64
   p.B = d->B, p.S = d->S, p.D = d->D, p.R = d->R;
   p.interleaved = d->interleaved ? 1 : 0;
   p.eps = d->eps;
+  p.inv_d = 1.f / static_cast<float>(d->D);
   p.part = nullptr;
   p.ctas[0] = p.ctas[1] = 0;
   if (const unsigned long long cap = debug_extent_limit())

@@ -140,14 +140,14 @@ kcg_status_t check_head_view(const HeadView& v, int elem_bytes) {
 }
 
 kcg_status_t encode_head_view(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const HeadView& v,
-                              CUtensorMapSwizzle swizzle) {
+                              CUtensorMapSwizzle swizzle, int rows) {
   const uint64_t dims[4] = {static_cast<uint64_t>(v.D), static_cast<uint64_t>(v.S), static_cast<uint64_t>(v.H),
                             static_cast<uint64_t>(v.B)};
   const uint64_t row = static_cast<uint64_t>(v.D) * elem_bytes;
   const uint64_t strides[3] = {v.S == 1 ? row : static_cast<uint64_t>(v.sr) * elem_bytes,
                                v.H == 1 ? row : static_cast<uint64_t>(v.sh) * elem_bytes,
                                v.B == 1 ? row : static_cast<uint64_t>(v.sb) * elem_bytes};
-  const uint32_t box[4] = {128u / static_cast<uint32_t>(elem_bytes), 128, 1, 1};
+  const uint32_t box[4] = {128u / static_cast<uint32_t>(elem_bytes), static_cast<uint32_t>(rows), 1, 1};
   return encode_tmap(map, dt, 4, v.base, dims, strides, box, swizzle);
 }
 

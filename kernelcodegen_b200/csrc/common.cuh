@@ -31,7 +31,7 @@ kcg_status_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, con
                          CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 // Tensor map of a [B, H, S, D] view (strides in elements; the innermost is 1): coordinates
-// (d, row, head, batch), boxes of 128 rows x 128 bytes, rows past S read as zero.  An extent of one
+// (d, row, head, batch), boxes of `rows` rows x 128 bytes, rows past S read as zero.  An extent of one
 // has no stride of its own; it is given one that the encoder accepts.
 struct HeadView {
   const void* base;
@@ -39,7 +39,7 @@ struct HeadView {
   int64_t sb, sh, sr;
 };
 kcg_status_t encode_head_view(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const HeadView& v,
-                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
+                              CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int rows = 128);
 // Whether a view can be read through such a map (16-byte rows) or written row by row.
 kcg_status_t check_head_view(const HeadView& v, int elem_bytes);
 // bytes from the first to one past the last element

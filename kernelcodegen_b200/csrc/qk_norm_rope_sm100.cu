@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
   constexpr unsigned GROUPS = RN_THREADS / LPR;
   __shared__ __align__(16) float weights[2][256];
   __shared__ float red[BWD ? RN_THREADS / 32 : 1][BWD ? 256 : 1];
+  if (BWD) griddep_launch_dependents();
   const int gl = threadIdx.x % LPR;
   const unsigned group = threadIdx.x / LPR;
   const int nv = p.D / N;
@@ -373,6 +374,7 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_c
   constexpr unsigned GROUPS = RN_THREADS / LPR;
   __shared__ float weights[2][256];
   __shared__ float red[BWD ? RN_THREADS / 32 : 1][BWD ? 256 : 1];
+  if (BWD) griddep_launch_dependents();
   const int gl = threadIdx.x % LPR;
   const unsigned group = threadIdx.x / LPR;
   const int half = p.R / 2;
@@ -510,23 +512,28 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_c
   }
 }
 
-// dw[i] = sum of the CTAs' partial sums, in a fixed order: 32 columns per CTA, 8 rows at a time.
-__global__ void __launch_bounds__(256) rope_weight_sum_kernel(const float* part, int first, int count, int D, float* dw0,
-                                                              int count1, float* dw1) {
-  __shared__ float red[8][33];
-  const int which = blockIdx.y;
-  float* dw = which ? dw1 : dw0;
+// dw[i] = sum of the CTAs' partial sums, in a fixed order: 32 columns per CTA, a warp per 32nd row.  Its
+// launch overlaps the kernel before it.
+__global__ void __launch_bounds__(1024) rope_weight_sum_kernel(const float* part, int count0, int count1, int D, float* dw0,
+                                                               float* dw1) {
+  __shared__ float red[32][33];
+  float* dw = blockIdx.y ? dw1 : dw0;
   if (!dw) return;
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), sub = threadIdx.x >> 5;
-  const int begin = which ? first + count : first, n = which ? count1 : count;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane;
+  const int n = blockIdx.y ? count1 : count0;
+  const float* rows = part + (blockIdx.y ? static_cast<long long>(count0) * D : 0) + col;
+  griddep_wait();
   float sum = 0.f;
-  if (col < D)
-    for (int i = sub; i < n; i += 8) sum += part[static_cast<long long>(begin + i) * D + col];
-  red[sub][threadIdx.x & 31] = sum;
+  if (col < D) {
+#pragma unroll 4
+    for (int i = sub; i < n; i += 32) sum += rows[static_cast<long long>(i) * D];
+  }
+  red[sub][lane] = sum;
   __syncthreads();
   if (sub == 0 && col < D) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) sum += red[k][threadIdx.x & 31];
+    for (int k = 1; k < 32; ++k) sum += red[k][lane];
     dw[col] = sum;
   }
 }
@@ -725,10 +732,18 @@ kcg_status_t qk_norm_rope_bwd_impl(const kcg_rope_desc* d, const void* dq_out, c
   st = d->dtype == KCG_F32 ? launch_rope<float, true>(p, d, vectors, stream)
                            : launch_rope<__nv_bfloat16, true>(p, d, vectors, stream);
   if (st != KCG_OK || !sums) return st;
-  rope_weight_sum_kernel<<<dim3(static_cast<unsigned>((d->D + 31) / 32), 2), 256, 0, stream>>>(
-      p.part, 0, p.ctas[0], d->D, dwq, p.ctas[1], d->Hk ? dwk : nullptr);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>((d->D + 31) / 32), 2);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  KCG_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_weight_sum_kernel, static_cast<const float*>(p.part), p.ctas[0], p.ctas[1],
+                                  static_cast<int>(d->D), dwq, d->Hk ? dwk : static_cast<float*>(nullptr)));
   g_launches.fetch_add(1);
-  KCG_CUDA_TRY(cudaGetLastError());
   return KCG_OK;
 }
 

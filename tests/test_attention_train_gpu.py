@@ -5,7 +5,8 @@ bf16; e = 2^-23, a truncating 32-bit addition):
   scores      D products of bf16 are exact in 32 bits, their sum is off by at most D e (|q|.|k|)
   P           relative: that times scale, plus 6e-6 (2^x to 2.6e-6, lse and the scaled score rounded)
   dP, delta   D e (|dO|.|v|), D e (|dO|.|O|)
-  P, dS       rounded to bf16 where they enter a product: u relative
+  P, dS       rounded to bf16 where they enter a product: u relative; the P in dS is itself a rounded one,
+              the bf16 one for dK (u more), fp16 of 2^15 P for dQ (2^-11 relative, 2^-40 absolute below 2^-29)
   sums        n e times the sum of magnitudes, n terms
   results     rounded to bf16: u relative
   underflow   2^x gives 0 below 2^-126 and the products may drop operands below it, so every P and dS
@@ -85,12 +86,14 @@ def check_backward(dout, q, k, v, out, lse, scale, causal, grads):
     relp = rel + 6e-6 + (at.abs() * E).nan_to_num(posinf=0)
     err_ds = p * (g.abs() @ vd.abs().transpose(2, 3) + (g * o).abs().sum(-1, keepdim=True)) * D * E + (relp + U) * ds.abs()
     err_ds = err_ds + TINY * (1 + dp.abs() + delta.abs())
+    err_dsq = err_ds + 2.0 ** -11 * ds.abs() + 2.0 ** -40 * (dp - delta).abs()
+    err_dsk = err_ds + U * ds.abs()
     err_p = (relp + U) * p + TINY
     ha = H // k.shape[1] * m          # terms of dk and dv
     fold = lambda t: t.view(t.shape[0], k.shape[1], -1, *t.shape[2:]).sum(2)  # noqa: E731
     want = [ds @ kd * scale, fold(ds.transpose(2, 3) @ qd) * scale, fold(p.transpose(2, 3) @ g)]
-    bound = [(err_ds + n * E * ds.abs()) @ kd.abs() * scale,
-             fold((err_ds + ha * E * ds.abs()).transpose(2, 3) @ qd.abs()) * scale,
+    bound = [(err_dsq + n * E * ds.abs()) @ kd.abs() * scale,
+             fold((err_dsk + ha * E * ds.abs()).transpose(2, 3) @ qd.abs()) * scale,
              fold((err_p + ha * E * p).transpose(2, 3) @ g.abs())]
     for name, got, w, b in zip(("dq", "dk", "dv"), grads, want, bound):
         check(got, w, 1.01 * b + U * w.abs() + TINY, name)

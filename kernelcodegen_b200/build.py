@@ -54,7 +54,9 @@ def build_bounds(force: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False, lib: Path = LIB_PATH, defines: list[str] | None = None,
           obj_subdir: str = "build") -> Path:
-    """Compile the library if it is missing or older than its sources."""
+    """Compile the library (and, with the normal one, the torch binding) if missing or older than its sources."""
+    if lib == LIB_PATH:
+        build_binding(force)
     if not force and not needs_build(lib):
         return lib
     nvcc = _nvcc()
@@ -83,6 +85,37 @@ def build(force: bool = False, verbose: bool = False, lib: Path = LIB_PATH, defi
         raise RuntimeError("link failed")
     os.replace(tmp, lib)
     return lib
+
+
+BINDING_PATH = PKG_DIR / "_torch_binding.so"
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile the torch binding of the attention training operators (csrc/torch_binding.cpp) against the
+    installed torch.  Plain C++; it calls the kernel library through addresses it is given at run time."""
+    src, header = CSRC / "torch_binding.cpp", PKG_DIR.parent / "include" / "kcg_capi.h"
+    if not force and BINDING_PATH.exists() and all(p.stat().st_mtime <= BINDING_PATH.stat().st_mtime for p in (src, header)):
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    cuda_inc = Path(_nvcc()).resolve().parents[1] / "include"
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in (*cpp_extension.include_paths(), cuda_inc, sysconfig.get_paths()["include"])),
+           str(src), "-o", str(tmp), "-L", str(torch_lib), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           *shared_libstdcxx(cxx)]
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout)
+        raise RuntimeError("building _torch_binding.so failed")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 HOST_LIB_PATH = PKG_DIR / "libkcg_runtime.so"
@@ -152,5 +185,6 @@ def compile_program(source: Path, output: Path, extra: list[str] | None = None) 
 if __name__ == "__main__":
     path = build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(path)
+    print(BINDING_PATH)
     print(build_bounds(force="--force" in sys.argv))
     print(build_host(force="--force" in sys.argv))

@@ -11,7 +11,6 @@ sm_100a kernels behind the C-ABI.  Nothing here falls back to torch math.
 from __future__ import annotations
 
 import ctypes
-import struct
 from typing import Optional, Sequence
 
 import torch
@@ -201,71 +200,24 @@ def fmha(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float = 1.
     return out
 
 
-# The operators below are called once per layer of a step, on short sequences too, where the host's part of a
-# call is most of its time: every property of a tensor is read once, and a descriptor is packed whole.
-_ATTN_PACK = struct.Struct("@8ifi24q")
-_ROPE_PACK = struct.Struct("@10iqfi20q")
-_POSITION_BITS = {torch.int32: 32, torch.int64: 64}
-_NO_STRIDES = (0, 0, 0)
-# the handle alone: torch.cuda.current_stream(dev).cuda_stream builds an object for it, 2 us of a 12 us call
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_native = None
 
 
-def _launch(dev: torch.device, fn, *args) -> int:
-    """fn(*args, stream) with `dev` current, on its current stream."""
-    index = dev.index
-    if torch.cuda.current_device() == index:
-        return fn(*args, _raw_stream(index))
-    with torch.cuda.device(dev):
-        return fn(*args, _raw_stream(index))
-
-
-def _view(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: torch.device):
-    """Batch, head and row stride of a [B, H, S, D] view, as the C-ABI takes them, of the tensor that is
-    expected."""
-    if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != dev:
-        raise RuntimeError("all tensors must live on the same device")
-    sb, sh, sr, sd = t.stride()
-    if sd != 1 and shape[3] != 1:
-        raise ValueError(f"{name} must have stride 1 in the last dimension")
-    return sb, sh, sr
-
-
-def _output(name: str, given: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device):
-    """An output [B, H, S, D] and its strides: a new contiguous tensor, or the one given."""
-    if given is not None:
-        return given, _view(name, given, shape, dtype, dev)
-    _, H, S, D = shape
-    strides = (H * S * D, S * D, D)
-    # (empty_strided takes half the host time of empty)
-    return torch.empty_strided(shape, (*strides, 1), dtype=dtype, device=dev), strides
-
-
-def _attn_views(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
-    """Checks Q, K and V of an attention call; (device, their shapes, their strides)."""
-    dev = q.device
-    if not q.is_cuda:
-        raise RuntimeError("kernelcodegen_b200 operators need CUDA tensors; there is no CPU path")
-    q_shape, k_shape = q.shape, k.shape
-    if len(q_shape) != 4 or len(k_shape) != 4 or k_shape != v.shape or q_shape[0] != k_shape[0] or q_shape[3] != k_shape[3]:
-        raise ValueError("expected Q [B,H,Sq,D] and K, V [B,Hkv,Skv,D]")
-    if not q.dtype is k.dtype is v.dtype is torch.bfloat16:
-        raise TypeError("Q, K, V must be bfloat16: the gradients' contractions have no float32 form")
-    if k_shape[1] == 0 or q_shape[1] % k_shape[1]:
-        raise ValueError("the number of query heads must be a multiple of the number of key/value heads")
-    bf16 = torch.bfloat16
-    return dev, q_shape, k_shape, (*_view("Q", q, q_shape, bf16, dev), *_view("K", k, k_shape, bf16, dev),
-                                   *_view("V", v, k_shape, bf16, dev))
-
-
-def _attn_desc(q_shape, k_shape, causal: bool, scale: float, strides) -> "capi.AttnDesc":
-    B, H, Sq, D = q_shape
-    return capi.AttnDesc.from_buffer_copy(_ATTN_PACK.pack(B, H, k_shape[1], Sq, k_shape[2], D, capi.KCG_BF16,
-                                                          1 if causal else 0, scale, 0, *strides))
+def _binding():
+    """The compiled binding of the attention training operators, bound to the library that is loaded."""
+    global _native
+    if _native is None:
+        try:
+            from . import _torch_binding as native
+        except ImportError as e:
+            raise ImportError("kernelcodegen_b200/_torch_binding is missing or does not load: build it with "
+                              "`python -m kernelcodegen_b200.build` (there is no fallback)") from e
+        lib = capi.load()
+        native.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "kcg_fmha_fwd_lse_launch", "kcg_fmha_bwd_workspace_bytes", "kcg_fmha_bwd_launch", "kcg_qk_norm_rope_launch",
+            "kcg_qk_norm_rope_bwd_workspace_bytes", "kcg_qk_norm_rope_bwd_launch")))
+        _native = native
+    return _native
 
 
 def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float = 1.0, causal: bool = False,
@@ -276,13 +228,7 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
     last dimension (heads of a packed projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may
     have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.
     O is contiguous unless `out` is given."""
-    dev, q_shape, k_shape, strides = _attn_views(q, k, v)
-    out, o = _output("out", out, q_shape, torch.bfloat16, dev)
-    B, H, Sq, _ = q_shape
-    lse = torch.empty_strided((B, H, Sq), (H * Sq, Sq, 1), dtype=torch.float32, device=dev)
-    d = _attn_desc(q_shape, k_shape, causal, scale, (*strides, *o, *_NO_STRIDES * 4))
-    st = _launch(dev, capi.load().kcg_fmha_fwd_lse_launch, d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                 lse.data_ptr())
+    st, out, lse = (_native or _binding()).fmha_with_lse(q, k, v, scale, causal, out)
     if st:
         capi.check(st, "kcg_fmha_fwd_lse_launch")
     return out, lse
@@ -296,89 +242,10 @@ def fmha_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     (call with the same scale and causal).  Views as there; the gradients are contiguous unless dq, dk or
     dv is given, e.g. as the heads of a packed gradient.  Outputs must not overlap one another or an
     input.  The same bits on every call: nothing is added up in an order that can change."""
-    dev, q_shape, k_shape, strides = _attn_views(q, k, v)
-    bf16 = torch.bfloat16
-    g = _view("dout", dout, q_shape, bf16, dev)
-    o = _view("out", out, q_shape, bf16, dev)
-    if lse.shape != q_shape[:3] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
-        raise ValueError("lse must be the contiguous float32 [B,H,Sq] tensor of fmha_with_lse")
-    dq, sq = _output("dq", dq, q_shape, bf16, dev)
-    dk, sk = _output("dk", dk, k_shape, bf16, dev)
-    dv, sv = _output("dv", dv, k_shape, bf16, dev)
-    d = _attn_desc(q_shape, k_shape, causal, scale, (*strides, *o, *g, *sq, *sk, *sv))
-    lib = capi.load()
-    # a buffer of this call alone, from the stream's allocator: two captured graphs never share it
-    ws_bytes = lib.kcg_fmha_bwd_workspace_bytes(d)
-    ws = torch.empty_strided((ws_bytes,), (1,), dtype=torch.uint8, device=dev)
-    st = _launch(dev, lib.kcg_fmha_bwd_launch, d, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                 lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes)
+    st, dq, dk, dv = (_native or _binding()).fmha_backward(dout, q, k, v, out, lse, scale, causal, dq, dk, dv)
     if st:
         capi.check(st, "kcg_fmha_bwd_launch")
     return dq, dk, dv
-
-
-def _rope_views(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
-    """Checks what both directions of qk_norm_rope take; (device, shapes of q and k, the descriptor up to
-    the strides, strides of q and k, pointers of weights, tables and positions)."""
-    q_shape, dtype, dev = q.shape, q.dtype, q.device
-    if len(q_shape) != 4:
-        raise ValueError("expected queries (and keys) as [B, heads, S, D]")
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
-        raise TypeError(f"unsupported dtype {dtype}: the kernels take float32 or bfloat16")
-    if not q.is_cuda:
-        raise RuntimeError("kernelcodegen_b200 operators need CUDA tensors; there is no CPU path")
-    B, H, S, D = q_shape
-    strides, k_shape = _view("q", q, q_shape, dtype, dev), None
-    if k is not None:
-        k_shape = k.shape
-        if len(k_shape) != 4 or k_shape[0] != B or k_shape[2] != S or k_shape[3] != D:
-            raise ValueError(f"k has shape {tuple(k_shape)}, expected [{B}, heads, {S}, {D}]")
-        strides += _view("k", k, k_shape, dtype, dev)
-    else:
-        if k_weight is not None:
-            raise ValueError("k_weight without keys")
-        strides += _NO_STRIDES
-    t_shape = cos.shape
-    if len(t_shape) != 2 or t_shape != sin.shape or 2 * t_shape[1] > D:
-        raise ValueError("cos and sin must be [positions, R / 2] with R <= D")
-    for t in (cos, sin):
-        if t.dtype is not torch.float32 or not t.is_contiguous():
-            raise TypeError("cos and sin must be contiguous float32 tables")
-        if t.device != dev:
-            raise RuntimeError("all tensors must live on the same device")
-    w_dtype = None
-    for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        if w_dtype is None:
-            w_dtype = w.dtype
-        if w.shape != (D,) or w.dtype is not w_dtype or not w.is_contiguous():
-            raise ValueError("the weights must be contiguous [D] tensors of one type")
-        if w.device != dev:
-            raise RuntimeError("all tensors must live on the same device")
-    pos_bits, pos = 32, (0, 0)
-    if positions is not None:
-        pos_bits = _POSITION_BITS.get(positions.dtype)
-        if pos_bits is None:
-            raise TypeError("positions must be int32 or int64")
-        p_shape = positions.shape
-        if p_shape == (B, S):
-            pos = positions.stride()
-        elif p_shape == (S,):
-            pos = (0, positions.stride(0))
-        else:
-            raise ValueError(f"positions must be [{S}] or [{B}, {S}]")
-        if positions.device != dev:
-            raise RuntimeError("all tensors must live on the same device")
-    elif S > t_shape[0]:
-        raise ValueError("more tokens than rows of the tables")
-    head = (B, S, H, k_shape[1] if k is not None else 0, D, 2 * t_shape[1], _dtype_code(dtype),
-            capi.KCG_F32 if w_dtype is None else _dtype_code(w_dtype), 1 if interleaved else 0, pos_bits, t_shape[0], eps, 0, *pos)
-    return dev, q_shape, k_shape, head, strides, (_ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), _ptr(positions))
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, *,
@@ -395,18 +262,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
     row's rotated entries NaN and sets `last_device_status()` to 11.
     The outputs are contiguous [B, heads, S, D] unless q_out / k_out is given (a slice of a key cache, or
     the input itself)."""
-    dev, q_shape, k_shape, head, strides, ptrs = _rope_views(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
-    dtype = q.dtype
-    q_out, yq = _output("q_out", q_out, q_shape, dtype, dev)
-    yk = _NO_STRIDES
-    if k is not None:
-        k_out, yk = _output("k_out", k_out, k_shape, dtype, dev)
-    elif k_out is not None:
-        raise ValueError("k_out without keys")
-    if q.numel() == 0 and (k is None or k.numel() == 0):
-        return q_out, k_out
-    d = capi.RopeDesc.from_buffer_copy(_ROPE_PACK.pack(*head, *strides, *yq, *yk, *_NO_STRIDES * 2))
-    st = _launch(dev, capi.load().kcg_qk_norm_rope_launch, d, q.data_ptr(), _ptr(k), *ptrs, q_out.data_ptr(), _ptr(k_out))
+    st, q_out, k_out = (_native or _binding()).qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
+                                                            q_out, k_out)
     if st:
         capi.check(st, "kcg_qk_norm_rope_launch")
     return q_out, k_out
@@ -422,30 +279,8 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
     it was called with.  The weights' gradients are float32 [D], summed over batch, heads and tokens in a
     fixed order (None for a weight that is None).  dq and dk are contiguous unless given; they may be
     dq_out and dk_out themselves."""
-    dev, q_shape, k_shape, head, strides, ptrs = _rope_views(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
-    dtype = q.dtype
-    if (dk_out is None) != (k is None) or (k is None and dk is not None):
-        raise ValueError("keys and their gradients go together")
-    gq, gk, sk = _view("dq_out", dq_out, q_shape, dtype, dev), _NO_STRIDES, _NO_STRIDES
-    dq, sq = _output("dq", dq, q_shape, dtype, dev)
-    if k is not None:
-        gk = _view("dk_out", dk_out, k_shape, dtype, dev)
-        dk, sk = _output("dk", dk, k_shape, dtype, dev)
-    empty = q.numel() == 0 and (k is None or k.numel() == 0)
-    dqw, dkw = (torch.empty_strided((q_shape[3],), (1,), dtype=torch.float32, device=dev) if w is not None else None
-                for w in (q_weight, k_weight))
-    if empty:
-        for w in (dqw, dkw):
-            if w is not None:
-                w.zero_()
-        return dq, dk, dqw, dkw
-    d = capi.RopeDesc.from_buffer_copy(_ROPE_PACK.pack(*head, *strides, *gq, *gk, *sq, *sk))
-    lib = capi.load()
-    # a buffer of this call alone, from the stream's allocator: two captured graphs never share it
-    ws_bytes = lib.kcg_qk_norm_rope_bwd_workspace_bytes(d) if dqw is not None or dkw is not None else 0
-    ws = torch.empty_strided((ws_bytes,), (1,), dtype=torch.uint8, device=dev) if ws_bytes else None
-    st = _launch(dev, lib.kcg_qk_norm_rope_bwd_launch, d, dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), *ptrs,
-                 dq.data_ptr(), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws), ws_bytes)
+    st, dq, dk, dqw, dkw = (_native or _binding()).qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, q_weight, k_weight,
+                                                                         positions, eps, interleaved, dq, dk)
     if st:
         capi.check(st, "kcg_qk_norm_rope_bwd_launch")
     return dq, dk, dqw, dkw

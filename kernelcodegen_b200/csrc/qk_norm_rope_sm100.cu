@@ -101,8 +101,9 @@ struct Unit {
       type = u >= p.units[0] ? 1 : 0;
       if (type) u -= p.units[0];
     }
-    const unsigned chunks = p.chunks[type], token = u / chunks;
-    h_first = static_cast<int>(u - token * chunks) * p.chunk[type];
+    // consecutive groups take consecutive tokens: their rows of a head are neighbours in the output
+    const unsigned tokens = static_cast<unsigned>(p.B) * p.S, run = u / tokens, token = u - run * tokens;
+    h_first = static_cast<int>(run) * p.chunk[type];
     b = static_cast<int>(token / p.S);
     s = static_cast<int>(token - static_cast<unsigned>(b) * p.S);
     n_heads = live ? min(p.chunk[type], p.heads[type] - h_first) : 0;
@@ -132,17 +133,26 @@ __device__ __forceinline__ float group_sum(float v) {
 
 __device__ __forceinline__ float2 swap2(float2 v) { return make_float2(v.y, v.x); }
 
-// The vector form: LPR lanes per row, two vectors per lane, U rows in flight
-// while U are computed.  The arithmetic is in pairs
-// of entries (packed fp32), the angles and weights multiplied into the lane's constants once per token:
+// The vector form: LPR lanes per row, two vectors per lane.  The rows on their way wait in shared memory, in
+// slots that one thread alone writes (asynchronous copies) and reads, DEPTH rows deep for every group: that
+// many registers would leave too few warps, and too few bytes in flight for the memory's latency (gradients
+// at 4 x 4096 x 40 x 128 in bf16: one row ahead in registers 3.9 TB/s, three in shared memory
+// 5.4).  The arithmetic is in pairs of entries (packed fp32), the angles and weights multiplied into the
+// lane's constants once per token:
 //   y_a = r (a * ca + mate_a * sa), with the mate of a vector's entries in the lane's other vector, or
 //   (neighbours) the other entry of the pair.
-template <typename T, int LPR, bool IL, bool BWD, int U>
+constexpr int rope_rows(bool bwd) { return bwd ? 1 : 2; }     // rows of a group that are computed together
+constexpr int rope_depth(bool bwd) { return bwd ? 3 : 2; }    // times as many are on their way
+constexpr int rope_slots(bool bwd) { return bwd ? 4 : 2; }    // vectors of a row per lane: x, and dy
+template <typename T, int LPR, bool IL, bool BWD>
 __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_constant__ RopeParams p) {
   constexpr int N = Vec<T>::N, P = N / 2;
   constexpr unsigned GROUPS = RN_THREADS / LPR;
+  constexpr int U = rope_rows(BWD), DEPTH = rope_depth(BWD), SLOTS = rope_slots(BWD);
   __shared__ __align__(16) float weights[2][256];
   __shared__ float red[BWD ? RN_THREADS / 32 : 1][BWD ? 256 : 1];
+  extern __shared__ __align__(16) uint4 rows[];             // [DEPTH][U][SLOTS][RN_THREADS]
+  const uint32_t slot0 = smem_u32(rows) + threadIdx.x * 16;
   if (BWD) griddep_launch_dependents();
   const int gl = threadIdx.x % LPR;
   const unsigned group = threadIdx.x / LPR;
@@ -150,8 +160,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
   // the lane's vectors
   const int hp = IL ? 0 : p.R / (2 * N);
   const bool mates = gl < hp;
-  const int va = mates ? gl : 2 * hp + 2 * (gl - hp);
-  const int vb = mates ? gl + hp : va + 1;
+  const int va = IL || mates ? gl : 2 * hp + 2 * (gl - hp);
+  const int vb = IL ? gl + LPR : mates ? gl + hp : va + 1;
   const bool has_a = va < nv, has_b = vb < nv;
   // whether the lane's vectors are rotated (R is a multiple of a vector)
   const bool rot_a = has_a && (IL ? va * N < p.R : mates), rot_b = has_b && (IL ? vb * N < p.R : mates);
@@ -186,26 +196,41 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
     w.y0 = un.offset(p.ys[un.type]);
     return w;
   };
-  uint4 xn[U][2], dn[BWD ? U : 1][2];   // the round that is on its way
-  auto load = [&](const Where& w, int h0) {
-    const long long xh = p.xs[w.type][1], dh = p.ds[w.type][1];
+  // the row that is asked for next: of unit ui, head hi of the run
+  unsigned ui = u0;
+  int hi = 0, to = 0;
+  Where wi = place(u0);
+  auto request = [&]() {
+    if (ui < end) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const bool on = h0 + k < w.n_heads;
-      xn[k][0] = xn[k][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (on && has_a) xn[k][0] = *reinterpret_cast<const uint4*>(w.x + (h0 + k) * xh + va * N);
-      if (on && has_b) xn[k][1] = *reinterpret_cast<const uint4*>(w.x + (h0 + k) * xh + vb * N);
-      if (BWD) {
-        dn[k][0] = dn[k][1] = make_uint4(0u, 0u, 0u, 0u);
-        if (on && has_a) dn[k][0] = *reinterpret_cast<const uint4*>(w.dy + (h0 + k) * dh + va * N);
-        if (on && has_b) dn[k][1] = *reinterpret_cast<const uint4*>(w.dy + (h0 + k) * dh + vb * N);
+      for (int k = 0; k < U; ++k) {
+        const bool on = hi + k < wi.n_heads;
+        const T* xr = wi.x + (hi + k) * p.xs[wi.type][1];
+        const uint32_t at = slot0 + (to * U + k) * (SLOTS * RN_THREADS * 16);
+        cp_async16(at, on && has_a ? xr + va * N : wi.x, on && has_a);
+        cp_async16(at + RN_THREADS * 16, on && has_b ? xr + vb * N : wi.x, on && has_b);
+        if (BWD) {
+          const T* dr = wi.dy + (hi + k) * p.ds[wi.type][1];
+          cp_async16(at + 2 * RN_THREADS * 16, on && has_a ? dr + va * N : wi.dy, on && has_a);
+          cp_async16(at + 3 * RN_THREADS * 16, on && has_b ? dr + vb * N : wi.dy, on && has_b);
+        }
+      }
+      hi += U;
+      if (hi >= rounds) {
+        hi = 0;
+        ui += step;
+        if (ui < end) wi = place(ui);
       }
     }
+    cp_async_commit();     // (an empty group past the end, so that the count stays)
+    to = to + 1 == DEPTH ? 0 : to + 1;
   };
-  Where un = place(u0);
-  load(un, 0);
+  Where un = wi;
+#pragma unroll
+  for (int k = 0; k < DEPTH - 1; ++k) request();
   stage_weights(p, weights);
   __syncthreads();
+  int from = 0;
   for (;;) {
     const int type = un.type;
     const long long yh = p.ys[type][1];
@@ -214,7 +239,7 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
     {
       const long long tr = un.tr;
       // angle of pair i of the lane: half-split, entry i of a with entry i of b; neighbours, first the P
-      // pairs of a, then those of b.  Either way consecutive entries of the tables.
+      // pairs of a, then those of b
       float2 c[P], sn[P];
       const float* ct = p.cs + tr * (p.R / 2) + va * (IL ? P : N);
       const float* st = p.sn + tr * (p.R / 2) + va * (IL ? P : N);
@@ -225,8 +250,9 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
         c[i] = rot ? make_float2(bad, bad) : make_float2(1.f, 1.f);
         sn[i] = rot ? make_float2(bad, bad) : make_float2(0.f, 0.f);
         if (rot && tr >= 0) {
-          c[i] = __ldg(reinterpret_cast<const float2*>(ct) + i);
-          sn[i] = __ldg(reinterpret_cast<const float2*>(st) + i);
+          const int at = IL && 2 * i >= P ? (vb - va) * P + 2 * i - P : 2 * i;
+          c[i] = __ldg(reinterpret_cast<const float2*>(ct + at));
+          sn[i] = __ldg(reinterpret_cast<const float2*>(st + at));
         }
       }
       float2 wa[P], wb[P];
@@ -261,24 +287,21 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
     const bool more = u0 + step < end;
     Where next = un;
     if (more) next = place(u0 + step);
+    if (more && next.tr >= 0) {     // the next token's angles, out of the way of its first row
+      prefetch_l1(p.cs + next.tr * (p.R / 2) + (rot_a ? va * (IL ? P : N) : 0));
+      prefetch_l1(p.sn + next.tr * (p.R / 2) + (rot_a ? va * (IL ? P : N) : 0));
+    }
     for (int h0 = 0; h0 < rounds; h0 += U) {
-      uint4 xv[U][2], dv[BWD ? U : 1][2];
-#pragma unroll
-      for (int k = 0; k < U; ++k)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          xv[k][j] = xn[k][j];
-          if (BWD) dv[k][j] = dn[k][j];
-        }
-      // the next round, of this token or of the group's next one, is on its way while this is computed
-      if (h0 + U < rounds) load(un, h0 + U);
-      else if (more) load(next, 0);
+      request();
+      cp_async_wait<DEPTH - 1>();
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const bool on = h0 + k < un.n_heads;
+        const uint32_t at = slot0 + (from * U + k) * (SLOTS * RN_THREADS * 16);
+        const uint4 xa = ld_shared_v4(at), xb = ld_shared_v4(at + RN_THREADS * 16);
         float2 a[P], bb[P], s2 = make_float2(0.f, 0.f);
-        Vec<T>::unpack(xv[k][0], a);
-        Vec<T>::unpack(xv[k][1], bb);
+        Vec<T>::unpack(xa, a);
+        Vec<T>::unpack(xb, bb);
 #pragma unroll
         for (int i = 0; i < P; ++i) s2 = fma2(bb[i], bb[i], fma2(a[i], a[i], s2));
         const float r = rsqrtf(group_sum<LPR>(s2.x + s2.y) * p.inv_d + p.eps);
@@ -292,8 +315,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
           }
         } else {
           float2 ga[P], gb[P], d2 = make_float2(0.f, 0.f);
-          Vec<T>::unpack(dv[k][0], ga);
-          Vec<T>::unpack(dv[k][1], gb);
+          Vec<T>::unpack(ld_shared_v4(at + 2 * RN_THREADS * 16), ga);
+          Vec<T>::unpack(ld_shared_v4(at + 3 * RN_THREADS * 16), gb);
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const float2 f = ga[i], g = gb[i];
@@ -324,14 +347,15 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
           }
         }
         if (on) {
-          const long long at = un.y0 + (h0 + k) * yh;
-          T* yr = static_cast<T*>(p.y[type]) + at;
-          if (has_a && bounds_ok((at + va * N) * sizeof(T), 16, p.y_extent[type], p.status, p.bounds_detail))
+          const long long to_row = un.y0 + (h0 + k) * yh;
+          T* yr = static_cast<T*>(p.y[type]) + to_row;
+          if (has_a && bounds_ok((to_row + va * N) * sizeof(T), 16, p.y_extent[type], p.status, p.bounds_detail))
             *reinterpret_cast<uint4*>(yr + va * N) = Vec<T>::pack(oa);
-          if (has_b && bounds_ok((at + vb * N) * sizeof(T), 16, p.y_extent[type], p.status, p.bounds_detail))
+          if (has_b && bounds_ok((to_row + vb * N) * sizeof(T), 16, p.y_extent[type], p.status, p.bounds_detail))
             *reinterpret_cast<uint4*>(yr + vb * N) = Vec<T>::pack(ob);
         }
       }
+      from = from + 1 == DEPTH ? 0 : from + 1;
     }
     if (!more) break;
     un = next;
@@ -558,14 +582,22 @@ void bwd_ctas(const kcg_rope_desc* d, int& q, int& k) {
   q = most - k;
 }
 
+template <typename T, int LPR, bool IL, bool BWD>
+kcg_status_t go_vec(const RopeParams& p, unsigned grid, cudaStream_t stream) {
+  constexpr int bytes = rope_depth(BWD) * rope_rows(BWD) * rope_slots(BWD) * RN_THREADS * 16;
+  auto kern = rope_vec_kernel<T, LPR, IL, BWD>;
+  static std::atomic<bool> allowed[64];
+  const kcg_status_t st = allow_smem(kern, bytes, allowed);
+  if (st == KCG_OK) kern<<<grid, RN_THREADS, bytes, stream>>>(p);
+  return st;
+}
 template <typename T, bool IL, bool BWD>
-void go_vec(const RopeParams& p, int lpr, unsigned grid, cudaStream_t stream) {
-  constexpr int U = BWD ? 1 : 2;
+kcg_status_t go_vec(const RopeParams& p, int lpr, unsigned grid, cudaStream_t stream) {
   switch (lpr) {
-    case 4: return rope_vec_kernel<T, 4, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
-    case 8: return rope_vec_kernel<T, 8, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
-    case 16: return rope_vec_kernel<T, 16, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
-    default: return rope_vec_kernel<T, 32, IL, BWD, U><<<grid, RN_THREADS, 0, stream>>>(p);
+    case 4: return go_vec<T, 4, IL, BWD>(p, grid, stream);
+    case 8: return go_vec<T, 8, IL, BWD>(p, grid, stream);
+    case 16: return go_vec<T, 16, IL, BWD>(p, grid, stream);
+    default: return go_vec<T, 32, IL, BWD>(p, grid, stream);
   }
 }
 template <typename T, bool BWD>
@@ -592,10 +624,10 @@ kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cu
   const int per_cta = RN_THREADS / (vec ? lpr : d->D <= 128 ? 16 : 32);
   const long long tokens = static_cast<long long>(d->B) * d->S, sms = device_sm_count();
   for (int t = 0; t < 2; ++t) {
-    // heads a group walks with one set of angles: as many as leave two groups' worth of work for
-    // every group that the SMs hold, at most 8
+    // heads a group walks with one set of angles: as many as leave work for every group that the SMs hold
+    // (two CTAs each), at most 8.  (3 x 777 tokens x 16 heads: 14.6 us with one head, 11.2 with four)
     int chunk = 1;
-    while (chunk < 8 && 2 * chunk <= p.heads[t] && tokens * p.heads[t] / (2 * chunk) >= sms * 8 * per_cta) chunk *= 2;
+    while (chunk < 8 && 2 * chunk <= p.heads[t] && tokens * p.heads[t] / (2 * chunk) >= sms * 2 * per_cta) chunk *= 2;
     const int chunks = p.heads[t] ? (p.heads[t] + chunk - 1) / chunk : 0;
     if (tokens * chunks > 0x3FFFFFFFll) return KCG_BAD_SHAPE;
     p.chunk[t] = chunk;
@@ -613,9 +645,10 @@ kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cu
     const long long want = (static_cast<long long>(p.units[0]) + p.units[1] + per_cta - 1) / per_cta, most = (vec ? 2 : 16) * sms;
     grid = static_cast<unsigned>(want < most ? want : most);
   }
+  kcg_status_t st = KCG_OK;
   if (!vec) go_pair<T, BWD>(p, grid, stream);
-  else if (d->interleaved) go_vec<T, true, BWD>(p, lpr, grid, stream);
-  else go_vec<T, false, BWD>(p, lpr, grid, stream);
+  else st = d->interleaved ? go_vec<T, true, BWD>(p, lpr, grid, stream) : go_vec<T, false, BWD>(p, lpr, grid, stream);
+  if (st != KCG_OK) return st;
   g_launches.fetch_add(1);
   KCG_CUDA_TRY(cudaGetLastError());
   return KCG_OK;

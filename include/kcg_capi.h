@@ -236,8 +236,10 @@ kcg_status_t kcg_fmha_fwd_launch(const kcg_fmha_desc* d, const void* Q, const vo
 
 /* Attention forward that also leaves what its gradient needs: O as above and
  * lse[b, h, i] = log sum_j exp(scale * q_i.k_j) over the visible keys (fp32, contiguous [B, H, Sq],
- * natural logarithm; -inf and O = 0 for a query that sees no key).  No counterpart in the reference,
- * which generates forward kernels only. */
+ * natural logarithm; -inf and O = 0 for a query that sees no key).  O must not overlap an input (equal
+ * pointers are KCG_BAD_ARGUMENT); the inputs must be finite wherever the tensors have an entry (a masked NaN
+ * still reaches the products it is part of).  No counterpart in the reference, which generates forward
+ * kernels only. */
 kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
                                      float* lse, void* stream);
 
@@ -246,8 +248,8 @@ kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, cons
  *   P_ij = exp(scale q_i.k_j - lse_i), delta_i = dO_i.O_i, dS_ij = P_ij (dO_i.v_j - delta_i),
  *   dV_j = sum_i P_ij dO_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j,
  * the sums of dK and dV over all query heads of the group.  Accumulation in fp32 in a fixed order (the
- * same bits on every call).  The outputs must not overlap one another or an input; the inputs must be
- * finite wherever the tensors have an entry (a masked NaN still reaches the products it is part of).
+ * same bits on every call).  The outputs must not overlap one another or an input (equal pointers are
+ * KCG_BAD_ARGUMENT); the inputs must be finite, as in the forward call.
  * Workspace: kcg_fmha_bwd_workspace_bytes, not shared by calls that may overlap. */
 size_t kcg_fmha_bwd_workspace_bytes(const kcg_attn_desc* d);
 kcg_status_t kcg_fmha_bwd_launch(const kcg_attn_desc* d, const void* dO, const void* Q, const void* K, const void* V,
@@ -360,7 +362,9 @@ kcg_status_t kcg_peer_wait_launch(const void* flags, int32_t n, int32_t stride_w
 kcg_status_t kcg_peer_wait_status(void);
 
 /* Reads (and clears) the status word of the current device that a kernel sets when one of
- * its bounded waits runs out; 0 = no timeout.  Synchronises the device. */
+ * its bounded waits runs out; 0 = no timeout.  Codes of another kind: 10 (bounds-checking build, below),
+ * 11 (kcg_qk_norm_rope_*: a position outside the tables), 12 (kcg_fmha_bwd_launch: shared memory did not
+ * start where the kernel needs it; nothing was computed).  Synchronises the device. */
 int kcg_last_device_status(void);
 
 /* Self-test of the bounded device-side wait: launches one thread that waits `iterations`

@@ -46,9 +46,11 @@
 //   kv    S / P: BN    dP / dS: BN    dV: D    dK: D
 //   q     S: BN        dP: BN         dQ: D    dS: 2 x BN / 2
 //
-// Measured (B200, bf16): see the table of cases in the design notes; 894 TFLOP/s of 5 products (1252 of the 7
-// that run) at 32 heads x 8192 causal, D = 128, where the power limit holds cuBLAS's own bf16 products to
-// 1384; one issuer instead of two 4 % less, descriptors rebuilt for every instruction 15 % less.
+// Measured (B200, bf16, causal, D = 128): 32 heads x 8192 1482 us, 927 TFLOP/s of 5 products (1298 of the 7 that
+// run) in short bursts, 1700 us in calls back to back for seconds, where the power limit holds cuBLAS's own
+// bf16 products to 1384 TFLOP/s; 16 heads x 4096 209 us.  One issuer instead of two: 1615 and 228 us.
+// D = 64, 2 x 32 heads x 4096 causal: 780 us, 440 TFLOP/s; one CTA per SM with 128-row tiles measures the same
+// within the noise of the clocks.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -175,8 +177,10 @@ __device__ __forceinline__ BwdItem item_at(const BwdParams& p, int idx) {
 constexpr int POLY_EIGHTHS = 3;
 __device__ __forceinline__ float2 exp2_share(int k, float2 x) {
   if (((k * 5) & 7) < POLY_EIGHTHS) {
-    x.x = fmaxf(x.x, -125.f);   // the polynomial's lower end: such a P is 2^-125, nothing in any sum
-    x.y = fmaxf(x.y, -125.f);
+    // the polynomial's lower end: such a P is 2^-125, nothing in any sum.  (A NaN stays one, and comes out as
+    // a number that bf16 rounds to infinity.)
+    x.x = fmax_nan(x.x, -125.f);
+    x.y = fmax_nan(x.y, -125.f);
     return ex2_quartic2(x);
   }
   x.x = ex2_approx(x.x);
@@ -588,7 +592,7 @@ __device__ __forceinline__ void run_item(const CUtensorMap* tmA0, const CUtensor
       }
       if (whole) {
         // scaled, rounded, and through shared memory (the tiles have been consumed): a thread's row written
-        // from here would be 32 rows to a store instruction, 4600 clocks for an item, and is 1300
+        // from here would be 32 rows to a store instruction
         const float f = is_v ? 1.f : p.scale;
         const uint32_t tile = base + (is_v ? BT * D * 2 : 0);
 #pragma unroll
@@ -844,6 +848,10 @@ kcg_status_t fmha_bwd_launch_impl(const kcg_attn_desc* d, const void* dO, const 
     if ((st = check_head_view(*v, 2)) != KCG_OK) return st;
   const BwdPlan n = plan_bwd(d);
   if (!ws || ws_bytes < n.bytes() || !aligned16(ws)) return KCG_BAD_WORKSPACE;
+  // an output over an input or another output: it would be written while other CTAs still read it
+  for (const void* x : {dO, Q, K, V, O})
+    if (x == dQ || x == dK || x == dV) return KCG_BAD_ARGUMENT;
+  if (dQ == dK || dQ == dV || dK == dV) return KCG_BAD_ARGUMENT;
   const long long ctas = n.kv_items * n.kv_split + n.q_items * n.q_split;
   if (ctas > 0x7FFFFFFFll || static_cast<long long>(d->H / d->Hkv) * n.n_qt > 0x3FFFFFFFll) return KCG_BAD_SHAPE;
   CUtensorMap tq, tk, tv, tdo;

@@ -413,12 +413,16 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       float mxg[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        mxg[g] = fmax3(__uint_as_float(sr[g][0]), __uint_as_float(sr[g][1]), __uint_as_float(sr[g][2]));
+        auto max3 = [](float a, float b, float d) { return LSE ? fmax3_nan(a, b, d) : fmax3(a, b, d); };
+        mxg[g] = max3(__uint_as_float(sr[g][0]), __uint_as_float(sr[g][1]), __uint_as_float(sr[g][2]));
 #pragma unroll
-        for (int i = 3; i < 31; i += 2) mxg[g] = fmax3(mxg[g], __uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]));
-        mxg[g] = fmaxf(mxg[g], __uint_as_float(sr[g][31]));
+        for (int i = 3; i < 31; i += 2) mxg[g] = max3(mxg[g], __uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]));
+        mxg[g] = max3(mxg[g], __uint_as_float(sr[g][31]), __uint_as_float(sr[g][31]));
       }
-      const float mx = fmaxf(fmaxf(mxg[0], mxg[1]), fmaxf(mxg[2], mxg[3]));
+      const float mx = LSE ? fmax_nan(fmax_nan(mxg[0], mxg[1]), fmax_nan(mxg[2], mxg[3]))
+                           : fmaxf(fmaxf(mxg[0], mxg[1]), fmaxf(mxg[2], mxg[3]));
+      // a NaN score makes the row's sum NaN, and so its lse and output (the polynomial's clamp would lose it)
+      if (LSE && mx != mx) l = mx;
       // lazy rescale (warp-uniform decision: the TMEM accesses below are warp-collective)
       const bool grow = (mx - m) * c > RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY);
       if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -509,8 +513,9 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     if (ok && row < p.Sq &&
         bounds_ok(off * (p.out_bf16 ? 2 : 4), static_cast<unsigned long long>(D) * (p.out_bf16 ? 2 : 4), p.o_extent,
                   p.status, p.bounds_detail)) {
-      const float inv = l > 1e-30f ? 1.f / l : 0.f;   // a row with no visible key sums to < 2^-100
-      if (LSE) p.lse[static_cast<size_t>(bh) * p.Sq + row] = l > 1e-30f ? (m * c + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+      // a row with no visible key sums to < 2^-100
+      const float inv = (LSE ? l <= 1e-30f : !(l > 1e-30f)) ? 0.f : 1.f / l;
+      if (LSE) p.lse[static_cast<size_t>(bh) * p.Sq + row] = l <= 1e-30f ? -INFINITY : (m * c + __log2f(l)) * 0.6931471805599453f;
       if (p.out_bf16) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.O) + off);
 #pragma unroll
@@ -767,6 +772,7 @@ kcg_status_t fmha_lse_launch_impl(const kcg_attn_desc* d, const void* Q, const v
   const HeadView vo{O, d->B, d->H, d->Sq, d->D, d->o[0], d->o[1], d->o[2]};
   for (const HeadView* v : {&vq, &vk, &vv, &vo})
     if ((st = check_head_view(*v, 2)) != KCG_OK) return st;
+  if (O == Q || O == K || O == V) return KCG_BAD_ARGUMENT;   // written while other CTAs still read it
   CUtensorMap tq, tk, tv;
   if ((st = encode_head_view(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vq)) != KCG_OK) return st;
   if ((st = encode_head_view(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vk)) != KCG_OK) return st;

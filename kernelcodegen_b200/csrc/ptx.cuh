@@ -335,16 +335,6 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 // registers -> TMEM: 32 lanes x 32 columns of 32 bits (thread t writes lane base+t)
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -469,6 +459,17 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
 
 // 3-input max and packed fp32x2 arithmetic (sm_100): halve the instruction count of the
 // softmax inner loops.
+// the same, a NaN being the largest
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -512,7 +513,7 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   return r;
 }
 
-// The same with a quartic for 2^f (relative error 2.6e-6): for sums and probabilities that are kept
+// The same with a quartic for 2^f (relative error 2.7e-6, and 4 roundings of 32 bits): for sums and probabilities that are kept
 // or subtracted in 32 bits (saved row statistics, the backward pass).  Same clamp as ex2_poly2.
 __device__ __forceinline__ float2 ex2_quartic2(float2 x) {
   constexpr float MAGIC = 12582912.f;

@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
         Vec<T>::unpack(xb, bb);
 #pragma unroll
         for (int i = 0; i < P; ++i) s2 = fma2(bb[i], bb[i], fma2(a[i], a[i], s2));
-        const float r = rsqrtf(group_sum<LPR>(s2.x + s2.y) * p.inv_d + p.eps);
+        const float ms = group_sum<LPR>(s2.x + s2.y) * p.inv_d + p.eps;
+        const float r = on ? rsqrtf(ms) : 0.f;     // (a row of zeros with an eps of zero would be 0 * inf)
         const float2 r2 = make_float2(r, r);
         float2 oa[P], ob[P];
         if (!BWD) {
@@ -472,7 +473,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_c
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(bb[k][i], bb[k][i], ss));
-        const float r = rsqrtf(group_sum<LPR>(ss) * p.inv_d + p.eps);
+        const float ms = group_sum<LPR>(ss) * p.inv_d + p.eps;
+        const float r = on ? rsqrtf(ms) : 0.f;
         float oa[NP], ob[NP];
         if (!BWD) {
 #pragma unroll
@@ -679,7 +681,7 @@ kcg_status_t fill(const kcg_rope_desc* d, const void* const (&x)[2], const int64
   for (int t = 0; t < 2; ++t) {
     const int heads = t ? d->Hk : d->H;
     p.heads[t] = heads;
-    p.x[t] = x[t], p.dy[t] = dy[t], p.y[t] = y[t], p.w[t] = w[t];
+    p.x[t] = x[t], p.dy[t] = dy[t], p.y[t] = y[t], p.w[t] = heads ? w[t] : nullptr;
     p.y_extent[t] = 0;
     if (!heads) continue;
     if (reinterpret_cast<uintptr_t>(w[t]) % ws) return KCG_BAD_ALIGN;

@@ -227,7 +227,8 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
     bfloat16 [B, H, S, D] views with any strides that are multiples of 16 bytes and stride 1 in the
     last dimension (heads of a packed projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may
     have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.
-    O is contiguous unless `out` is given."""
+    O is contiguous unless `out` is given (not over an input).  All entries must be finite, those that no
+    query sees too: they take part in the products with weight zero."""
     st, out, lse = (_native or _binding()).fmha_with_lse(q, k, v, scale, causal, out)
     if st:
         capi.check(st, "kcg_fmha_fwd_lse_launch")

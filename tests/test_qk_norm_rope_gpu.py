@@ -202,6 +202,38 @@ def test_rows_of_zeros_and_extremes(cuda_device):
     check(dq, dx, bound, "dq")
 
 
+def test_eps_of_zero(cuda_device):
+    """No row is zero, so nothing is infinite: rows that a group of lanes has nothing to do for included."""
+    from kernelcodegen_b200 import ops
+
+    for S, H, D, R, dtype in ((5, 3, 64, 64, torch.bfloat16), (5, 3, 64, 64, torch.float32), (5, 3, 66, 50, torch.bfloat16), (13001, 3, 64, 64, torch.bfloat16)):
+        q, w = make((1, H, S, D), 1, dtype), make((D,), 2, dtype)
+        cos, sin = tables(S, R)
+        c, s = angles(cos, sin, None, 1, S)
+        y, _ = ops.qk_norm_rope(q, None, cos, sin, q_weight=w, eps=0.0)
+        check(y, *forward(q, w, c, s, R, 0.0, False), "q")
+        dy = make(q.shape, 3, dtype)
+        dq, _, dw, _ = ops.qk_norm_rope_backward(dy, None, q, None, cos, sin, q_weight=w, eps=0.0)
+        dx, bound, dwant, wbound = backward(dy, q, w, c, s, R, 0.0, False)
+        check(dq, dx, bound, "dq")
+        check(dw, dwant, wbound, "dw")
+
+
+def test_rows_further_apart_than_32_bits(cuda_device):
+    from kernelcodegen_b200 import ops
+
+    S, H, D = 70, 3, 64
+    room = torch.empty(2 ** 31 + 4 * H * S * D, device="cuda", dtype=torch.bfloat16)
+    q, y, dy, dq = (room.as_strided((2, H, S, D), (2 ** 31, D, H * D, 1), i * H * S * D) for i in range(4))
+    q.copy_(make((2, H, S, D), 1, torch.bfloat16))
+    dy.copy_(make((2, H, S, D), 2, torch.bfloat16))
+    cos, sin = tables(S, D)
+    ops.qk_norm_rope(q, None, cos, sin, q_out=y)
+    assert torch.equal(y, ops.qk_norm_rope(q.contiguous(), None, cos, sin)[0])
+    ops.qk_norm_rope_backward(dy, None, q, None, cos, sin, dq=dq)
+    assert torch.equal(dq, ops.qk_norm_rope_backward(dy.contiguous(), None, q.contiguous(), None, cos, sin)[0])
+
+
 @pytest.mark.parametrize("D,R", [(64, 32), (64, 18)])
 def test_a_position_outside_the_tables_is_reported(cuda_device, D, R):
     """Its rotated entries are NaN, the others and the other rows are what they should be."""

@@ -108,7 +108,7 @@ def build_binding(force: bool = False) -> Path:
     cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{p}" for p in (*cpp_extension.include_paths(), cuda_inc, sysconfig.get_paths()["include"])),
-           str(src), "-o", str(tmp), "-L", str(torch_lib), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           str(src), "-o", str(tmp), "-L", str(torch_lib), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            *shared_libstdcxx(cxx)]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if res.returncode != 0:

@@ -6,7 +6,8 @@
 // the C-ABI of include/kcg_capi.h: the functions are handed over as addresses once (bind), so that the
 // library the process has loaded, the bounds-checking build included, is the one that is called.
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty_strided.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -79,7 +80,7 @@ Tensor contiguous(at::IntArrayRef shape, at::ScalarType dtype, at::Device dev) {
     strides[i] = n;
     n *= shape[i] > 0 ? shape[i] : 1;
   }
-  return at::empty_strided(shape, at::IntArrayRef(strides.data(), shape.size()), at::TensorOptions().dtype(dtype).device(dev));
+  return at::detail::empty_strided_cuda(shape, at::IntArrayRef(strides.data(), shape.size()), dtype, dev);
 }
 
 // An output view: the one given, checked, or a new contiguous tensor.
@@ -160,9 +161,9 @@ std::tuple<int, Tensor, Tensor, Tensor> fmha_backward(const Tensor& dout, const 
   const c10::cuda::CUDAGuard guard(a.dev);
   // a buffer of this call alone, from the stream's allocator: two captured graphs never share it
   const size_t bytes = bwd_bytes(&a.d);
-  Tensor ws = contiguous({static_cast<int64_t>(bytes)}, at::kByte, a.dev);
+  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   const int st = bwd(&a.d, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                     static_cast<const float*>(lse.data_ptr()), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), bytes,
+                     static_cast<const float*>(lse.data_ptr()), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.get(), bytes,
                      c10::cuda::getCurrentCUDAStream(a.dev.index()).stream());
   return {st, dq, dk, dv};
 }
@@ -265,7 +266,7 @@ std::tuple<int, Tensor, Opt, Opt, Opt> qk_norm_rope_backward(const Tensor& dq_ou
   Rope r = rotation(q, k, cos, sin, wq, wk, positions, eps, interleaved);
   if (dk_out.has_value() != k.has_value() || (!k && dk_)) bad_value("keys and their gradients go together");
   put(r.d.q_out, view("dq_out", dq_out, r.q, r.dtype, r.dev));
-  Tensor dq, dk, dwq, dwk, ws;
+  Tensor dq, dk, dwq, dwk;
   put(r.d.d_q, output("dq", dq_, r.q, r.dtype, r.dev, dq));
   if (k) {
     put(r.d.k_out, view("dk_out", *dk_out, r.k, r.dtype, r.dev));
@@ -281,9 +282,10 @@ std::tuple<int, Tensor, Opt, Opt, Opt> qk_norm_rope_backward(const Tensor& dq_ou
     const c10::cuda::CUDAGuard guard(r.dev);
     // a buffer of this call alone, from the stream's allocator: two captured graphs never share it
     const size_t bytes = wq || wk ? rope_bwd_bytes(&r.d) : 0;
-    if (bytes) ws = contiguous({static_cast<int64_t>(bytes)}, at::kByte, r.dev);
+    c10::DataPtr ws;
+    if (bytes) ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
     st = rope_bwd(&r.d, dq_out.data_ptr(), data(dk_out), q.data_ptr(), data(k), data(wq), data(wk), cos.data_ptr(), sin.data_ptr(),
-                  data(positions), dq.data_ptr(), data(dk), static_cast<float*>(data(dwq)), static_cast<float*>(data(dwk)), data(ws),
+                  data(positions), dq.data_ptr(), data(dk), static_cast<float*>(data(dwq)), static_cast<float*>(data(dwk)), ws.get(),
                   bytes, c10::cuda::getCurrentCUDAStream(r.dev.index()).stream());
   }
   return {st, dq, k ? Opt(dk) : Opt(), wq ? Opt(dwq) : Opt(), wk ? Opt(dwk) : Opt()};

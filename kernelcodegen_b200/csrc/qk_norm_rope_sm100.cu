@@ -625,11 +625,27 @@ kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cu
   while (2 * lpr < nv) lpr *= 2;
   const int per_cta = RN_THREADS / (vec ? lpr : d->D <= 128 ? 16 : 32);
   const long long tokens = static_cast<long long>(d->B) * d->S, sms = device_sm_count();
+  // Heads a group walks with one set of angles, at most 8.  Vector form: the length whose rounds over all groups
+  // that the SMs hold (two CTAs each) take the fewest rows, a run counting one more for its start.  (3 x 777 tokens x
+  // 16 heads of 80 in fp32: 4 heads 6.1 us, 8 heads 8.2; 1500 x 40 of 128 in bf16: 4 heads 8.4, 8 heads 6.9.)
+  // Pair form: as long as every group still has work (backward, 2000 x 16 of 96: 2 heads 14.1 us, 4 heads 18.0).
+  auto runs = [&](int t, int c) { return tokens * ((p.heads[t] + c - 1) / c); };
+  auto rows = [&](int t, int c) {
+    const long long units = BWD ? runs(t, c) : runs(0, c) + runs(1, c), groups = per_cta * (BWD ? p.ctas[t] : 2 * sms);
+    constexpr int U = rope_rows(BWD);
+    return (units + groups - 1) / groups * ((c + U - 1) / U * U + 1);
+  };
   for (int t = 0; t < 2; ++t) {
-    // heads a group walks with one set of angles: as many as leave work for every group that the SMs hold
-    // (two CTAs each), at most 8.  (3 x 777 tokens x 16 heads: 14.6 us with one head, 11.2 with four)
     int chunk = 1;
-    while (chunk < 8 && 2 * chunk <= p.heads[t] && tokens * p.heads[t] / (2 * chunk) >= sms * 2 * per_cta) chunk *= 2;
+    if (!p.heads[t]) {
+      // (no such tensor)
+    } else if (vec) {
+      for (int c = 2; c <= 8; c *= 2)
+        if (rows(t, c) < rows(t, chunk)) chunk = c;
+    } else {
+      while (chunk < 8 && tokens * (p.heads[0] + p.heads[1]) / (2 * chunk) >= sms * 2 * per_cta) chunk *= 2;
+    }
+    if (chunk > p.heads[t]) chunk = p.heads[t] ? p.heads[t] : 1;
     const int chunks = p.heads[t] ? (p.heads[t] + chunk - 1) / chunk : 0;
     if (tokens * chunks > 0x3FFFFFFFll) return KCG_BAD_SHAPE;
     p.chunk[t] = chunk;

@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -295,8 +296,9 @@ std::tuple<int, Tensor, Opt, Opt, Opt> qk_norm_rope_backward(const Tensor& dq_ou
 
 PYBIND11_MODULE(_torch_binding, m) {
   m.def("bind", &bind);
-  m.def("fmha_with_lse", &fmha_with_lse);
-  m.def("fmha_backward", &fmha_backward);
-  m.def("qk_norm_rope", &qk_norm_rope);
-  m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
+  // (wrapped: torch's own errors, out of memory among them, keep their Python types)
+  m.def("fmha_with_lse", torch::wrap_pybind_function(fmha_with_lse));
+  m.def("fmha_backward", torch::wrap_pybind_function(fmha_backward));
+  m.def("qk_norm_rope", torch::wrap_pybind_function(qk_norm_rope));
+  m.def("qk_norm_rope_backward", torch::wrap_pybind_function(qk_norm_rope_backward));
 }

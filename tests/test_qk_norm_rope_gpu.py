@@ -202,6 +202,16 @@ def test_rows_of_zeros_and_extremes(cuda_device):
     check(dq, dx, bound, "dq")
 
 
+def test_out_of_memory_is_torch_s_error(cuda_device):
+    """An output of 512 GB cannot be had: the caller sees what any allocation would raise."""
+    from kernelcodegen_b200 import ops
+
+    q = torch.ones((1, 1, 1, 256), device="cuda", dtype=torch.bfloat16).expand(1, 1024, 2 ** 20, 256)
+    cos, sin = tables(4, 256)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.qk_norm_rope(q, None, cos, sin, positions=torch.zeros((1,), device="cuda", dtype=torch.int32).expand(2 ** 20))
+
+
 def test_eps_of_zero(cuda_device):
     """No row is zero, so nothing is infinite: rows that a group of lanes has nothing to do for included."""
     from kernelcodegen_b200 import ops

@@ -628,8 +628,6 @@ kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cu
   // Heads a group walks with one set of angles, at most 8.  Vector form: the length whose rounds over all groups
   // that the SMs hold (two CTAs each) take the fewest rows, a run counting one more for its start.  (3 x 777 tokens x
   // 16 heads of 80 in fp32: 4 heads 6.1 us, 8 heads 8.2; 1500 x 40 of 128 in bf16: 4 heads 8.4, 8 heads 6.9.)
-  // The gradients of many tokens, eight rounds or more, keep to 4 heads, which is what the memory takes best
-  // (4 x 4096 tokens x 40 x 128 in bf16: 82.5 us, 8 heads 90, 2 heads 94; forward 4 heads 58.5, 8 heads 57.3).
   // Pair form: as long as every group still has work (backward, 2000 x 16 of 96: 2 heads 14.1 us, 4 heads 18.0).
   auto runs = [&](int t, int c) { return tokens * ((p.heads[t] + c - 1) / c); };
   auto rows = [&](int t, int c) {
@@ -642,8 +640,7 @@ kcg_status_t launch_rope(RopeParams& p, const kcg_rope_desc* d, bool vectors, cu
     if (!p.heads[t]) {
       // (no such tensor)
     } else if (vec) {
-      const int longest = BWD && rows(t, 4) >= 8 * (4 + 1) ? 4 : 8;
-      for (int c = 2; c <= longest; c *= 2)
+      for (int c = 2; c <= 8; c *= 2)
         if (rows(t, c) < rows(t, chunk)) chunk = c;
     } else {
       while (chunk < 8 && tokens * (p.heads[0] + p.heads[1]) / (2 * chunk) >= sms * 2 * per_cta) chunk *= 2;

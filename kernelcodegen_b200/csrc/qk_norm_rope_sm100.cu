@@ -137,7 +137,7 @@ __device__ __forceinline__ float2 swap2(float2 v) { return make_float2(v.y, v.x)
 // slots that one thread alone writes (asynchronous copies) and reads, DEPTH rows deep for every group: that
 // many registers would leave too few warps, and too few bytes in flight for the memory's latency (gradients
 // at 4 x 4096 x 40 x 128 in bf16: one row ahead in registers 3.9 TB/s, three in shared memory
-// 5.4).  The arithmetic is in pairs of entries (packed fp32), the angles and weights multiplied into the
+// 5.6).  The arithmetic is in pairs of entries (packed fp32), the angles and weights multiplied into the
 // lane's constants once per token:
 //   y_a = r (a * ca + mate_a * sa), with the mate of a vector's entries in the lane's other vector, or
 //   (neighbours) the other entry of the pair.

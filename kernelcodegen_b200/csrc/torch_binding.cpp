@@ -2,7 +2,7 @@
 // argument checks, outputs, workspace, descriptor and launch of one call in one crossing.
 //
 // A call of these operators on one short sequence is host time and little else: through ctypes, with
-// every tensor property read from Python, it takes 15 to 28 us, and 7 to 12 this way.  The kernels stay behind
+// every tensor property read from Python, it takes 15 to 28 us, and 6 to 10 this way.  The kernels stay behind
 // the C-ABI of include/kcg_capi.h: the functions are handed over as addresses once (bind), so that the
 // library the process has loaded, the bounds-checking build included, is the one that is called.
 #include <ATen/core/Tensor.h>

@@ -116,9 +116,19 @@ kcg_status_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, con
     estr[i] = 1;
   }
   for (int i = 0; i + 1 < rank; ++i) gstrides[i] = strides_bytes[i];
-  CUresult r = fn(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides,
-                  gbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread's first CUDA call (an autograd worker's, for one): a driver call does not bring the thread its
+    // device's context as the runtime's calls do, and setting the device does.
+    int dev = 0;
+    KCG_CUDA_TRY(cudaGetDevice(&dev));
+    KCG_CUDA_TRY(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     std::fprintf(stderr, "kcg: cuTensorMapEncodeTiled failed with CUresult %d\n",
                  static_cast<int>(r));

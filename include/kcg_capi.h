@@ -270,7 +270,7 @@ kcg_status_t kcg_qk_norm_rope_launch(const kcg_rope_desc* d, const void* q, cons
 /* Its gradients, from those of the outputs and the inputs of the forward call: dq, dk (which may be the
  * same views as dq_out, dk_out or as q, k), and the weights' [D] in fp32 (dq_weight / dk_weight NULL =
  * not wanted; otherwise the workspace of kcg_qk_norm_rope_bwd_workspace_bytes, not shared by calls that
- * may overlap).  Sums in a fixed order. */
+ * may overlap).  Sums in a fixed order; dk_weight is zero where there are no key heads. */
 size_t kcg_qk_norm_rope_bwd_workspace_bytes(const kcg_rope_desc* d);
 kcg_status_t kcg_qk_norm_rope_bwd_launch(const kcg_rope_desc* d, const void* dq_out, const void* dk_out, const void* q,
                                          const void* k, const void* q_weight, const void* k_weight, const void* cos,

@@ -538,8 +538,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_c
   }
 }
 
-// dw[i] = sum of the CTAs' partial sums, in a fixed order: 32 columns per CTA, a warp per 32nd row.  Its
-// launch overlaps the kernel before it.
+// dw[i] = sum of the CTAs' partial sums, in a fixed order (zero where there are none: no key heads): 32 columns per
+// CTA, a warp per 32nd row.  Its launch overlaps the kernel before it.
 __global__ void __launch_bounds__(1024) rope_weight_sum_kernel(const float* part, int count0, int count1, int D, float* dw0,
                                                                float* dw1) {
   __shared__ float red[32][33];
@@ -774,7 +774,7 @@ kcg_status_t qk_norm_rope_bwd_impl(const kcg_rope_desc* d, const void* dq_out, c
   st = fill(d, {q, k}, {d->q, d->k}, {dq_out, dk_out}, {d->q_out, d->k_out}, {dq, dk}, {d->d_q, d->d_k}, {wq, wk}, cs, sn, pos,
             p, vectors);
   if (st != KCG_OK) return st;
-  const bool sums = dwq || (dwk && d->Hk);
+  const bool sums = dwq || dwk;
   if (sums) {
     if (!ws || ws_bytes < qk_norm_rope_bwd_workspace_impl(d) || !aligned16(ws)) return KCG_BAD_WORKSPACE;
     p.part = static_cast<float*>(ws);
@@ -793,7 +793,7 @@ kcg_status_t qk_norm_rope_bwd_impl(const kcg_rope_desc* d, const void* dq_out, c
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   KCG_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_weight_sum_kernel, static_cast<const float*>(p.part), p.ctas[0], p.ctas[1],
-                                  static_cast<int>(d->D), dwq, d->Hk ? dwk : static_cast<float*>(nullptr)));
+                                  static_cast<int>(d->D), dwq, dwk));
   g_launches.fetch_add(1);
   return KCG_OK;
 }

@@ -14,6 +14,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
+#include <limits>
 #include <optional>
 
 #include "../../include/kcg_capi.h"
@@ -101,6 +102,7 @@ struct Attn {
   kcg_attn_desc d{};
   at::Device dev{at::kCUDA, 0};
   Shape q, k;
+  bool empty;      // no query, or no key: nothing to launch
 };
 
 Attn attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal) {
@@ -113,7 +115,7 @@ Attn attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, 
   const auto bf16 = at::kBFloat16;
   if (q.scalar_type() != bf16 || k.scalar_type() != bf16 || v.scalar_type() != bf16)
     bad_type("Q, K, V must be bfloat16: the gradients' contractions have no float32 form");
-  if (a.k[1] == 0 || a.q[1] % a.k[1])
+  if (a.k[1] == 0 ? a.q[1] != 0 : a.q[1] % a.k[1] != 0)
     bad_value("the number of query heads must be a multiple of the number of key/value heads");
   for (const int64_t n : {a.q[0], a.q[1], a.q[2], a.k[2]})
     if (n > INT32_MAX) bad_value("an extent does not fit 32 bits");
@@ -129,7 +131,14 @@ Attn attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, 
   put(a.d.q, view("Q", q, a.q, bf16, a.dev));
   put(a.d.k, view("K", k, a.k, bf16, a.dev));
   put(a.d.v, view("V", v, a.k, bf16, a.dev));
+  a.empty = q.numel() == 0 || k.numel() == 0;
   return a;
+}
+
+// A call without queries or keys is checked like any other: the status that it would have with extents of one.
+int check_empty(kcg_attn_desc d) {
+  for (int32_t* n : {&d.B, &d.H, &d.Hkv, &d.Sq, &d.Skv}) *n = 1;
+  return bwd_bytes(&d) ? KCG_OK : fwd_lse(&d, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
 }
 
 std::tuple<int, Tensor, Tensor> fmha_with_lse(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal,
@@ -139,6 +148,12 @@ std::tuple<int, Tensor, Tensor> fmha_with_lse(const Tensor& q, const Tensor& k, 
   put(a.d.o, output("out", given, a.q, at::kBFloat16, a.dev, out));
   Tensor lse = contiguous({a.q[0], a.q[1], a.q[2]}, at::kFloat, a.dev);
   const c10::cuda::CUDAGuard guard(a.dev);
+  if (a.empty) {
+    // a query that sees no key
+    const int st = check_empty(a.d);
+    if (st == KCG_OK) out.zero_(), lse.fill_(-std::numeric_limits<float>::infinity());
+    return {st, out, lse};
+  }
   const int st = fwd_lse(&a.d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), static_cast<float*>(lse.data_ptr()),
                          c10::cuda::getCurrentCUDAStream(a.dev.index()).stream());
   return {st, out, lse};
@@ -160,6 +175,11 @@ std::tuple<int, Tensor, Tensor, Tensor> fmha_backward(const Tensor& dout, const 
   put(a.d.d_k, output("dk", dk_, a.k, bf16, a.dev, dk));
   put(a.d.d_v, output("dv", dv_, a.k, bf16, a.dev, dv));
   const c10::cuda::CUDAGuard guard(a.dev);
+  if (a.empty) {
+    const int st = check_empty(a.d);
+    if (st == KCG_OK) dq.zero_(), dk.zero_(), dv.zero_();
+    return {st, dq, dk, dv};
+  }
   // a buffer of this call alone, from the stream's allocator: two captured graphs never share it
   const size_t bytes = bwd_bytes(&a.d);
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
@@ -250,6 +270,10 @@ std::tuple<int, Tensor, Opt> qk_norm_rope(const Tensor& q, const Opt& k, const T
   if (!k && k_out_) bad_value("k_out without keys");
   Tensor q_out, k_out;
   put(r.d.q_out, output("q_out", q_out_, r.q, r.dtype, r.dev, q_out));
+  if (!r.empty && r.d.H == 0) {      // keys alone: they take the queries' place
+    const auto keys = qk_norm_rope(*k, {}, cos, sin, wk, {}, positions, eps, interleaved, k_out_, {});
+    return {std::get<0>(keys), q_out, std::get<1>(keys)};
+  }
   if (k) put(r.d.k_out, output("k_out", k_out_, r.k, r.dtype, r.dev, k_out));
   int st = KCG_OK;
   if (!r.empty) {
@@ -269,6 +293,11 @@ std::tuple<int, Tensor, Opt, Opt, Opt> qk_norm_rope_backward(const Tensor& dq_ou
   put(r.d.q_out, view("dq_out", dq_out, r.q, r.dtype, r.dev));
   Tensor dq, dk, dwq, dwk;
   put(r.d.d_q, output("dq", dq_, r.q, r.dtype, r.dev, dq));
+  if (!r.empty && r.d.H == 0) {      // keys alone: they take the queries' place
+    const auto keys = qk_norm_rope_backward(*dk_out, {}, *k, {}, cos, sin, wk, {}, positions, eps, interleaved, dk_, {});
+    if (wq) dwq = contiguous({r.q[3]}, at::kFloat, r.dev).zero_();
+    return {std::get<0>(keys), dq, std::get<1>(keys), wq ? Opt(dwq) : Opt(), std::get<3>(keys)};
+  }
   if (k) {
     put(r.d.k_out, view("dk_out", *dk_out, r.k, r.dtype, r.dev));
     put(r.d.d_k, output("dk", dk_, r.k, r.dtype, r.dev, dk));

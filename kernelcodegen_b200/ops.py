@@ -226,7 +226,8 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
     exp(scale q_i.k_j) in float32 [B, H, Sq] (-inf, and O = 0, for a query that sees no key).
     bfloat16 [B, H, S, D] views with any strides that are multiples of 16 bytes and stride 1 in the
     last dimension (heads of a packed projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may
-    have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.
+    have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.  Any other
+    extent may be zero: with no keys O = 0 and lse = -inf.
     O is contiguous unless `out` is given (not over an input).  All entries must be finite, those that no
     query sees too: they take part in the products with weight zero."""
     st, out, lse = (_native or _binding()).fmha_with_lse(q, k, v, scale, causal, out)
@@ -242,7 +243,8 @@ def fmha_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     """(dQ, dK, dV) of `fmha_with_lse`, from the gradient of its O and the `out` and `lse` it returned
     (call with the same scale and causal).  Views as there; the gradients are contiguous unless dq, dk or
     dv is given, e.g. as the heads of a packed gradient.  Outputs must not overlap one another or an
-    input.  The same bits on every call: nothing is added up in an order that can change."""
+    input.  The same bits on every call: nothing is added up in an order that can change.  Zero where an
+    extent of zero leaves nothing to sum."""
     st, dq, dk, dv = (_native or _binding()).fmha_backward(dout, q, k, v, out, lse, scale, causal, dq, dk, dv)
     if st:
         capi.check(st, "kcg_fmha_bwd_launch")
@@ -257,7 +259,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
     """What attention wants done to queries and keys first, in one pass: every head row x becomes
     x / sqrt(mean(x^2) + eps) * weight (weight [D], ones when None), and the pairs (a, b) of its first
     R entries are rotated to (a cos - b sin, b cos + a sin).  q is a [B, H, S, D] view, k a [B, Hk, S, D]
-    one or None, float32 or bfloat16, any strides but 1 in the last dimension; D even, at most 256.
+    one or None, float32 or bfloat16, any strides but 1 in the last dimension; D even, at most 256; batch, heads
+    and S may be zero.
     cos, sin: float32 [positions, R / 2] tables; pairs are (i, i + R/2), or (2i, 2i + 1) if `interleaved`.
     positions: int32 or int64 [S] or [B, S], None for 0..S-1; a position outside the tables makes the
     row's rotated entries NaN and sets `last_device_status()` to 11.

@@ -421,8 +421,9 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
       const float mx = LSE ? fmax_nan(fmax_nan(mxg[0], mxg[1]), fmax_nan(mxg[2], mxg[3]))
                            : fmaxf(fmaxf(mxg[0], mxg[1]), fmaxf(mxg[2], mxg[3]));
-      // a NaN score makes the row's sum NaN, and so its lse and output (the polynomial's clamp would lose it)
-      if (LSE && mx != mx) l = mx;
+      // a NaN score, or one that overflows 32 bits (scaled or not: inf - inf below), makes the row's sum NaN, and so
+      // its lse and output (the polynomial's clamp would lose it, and a scaled overflow every other column's too)
+      if (LSE && !(mx * c < INFINITY)) l = __int_as_float(0x7FC00000);
       // lazy rescale (warp-uniform decision: the TMEM accesses below are warp-collective)
       const bool grow = (mx - m) * c > RESCALE_LOG2 || (m == -INFINITY && mx != -INFINITY);
       if (__any_sync(0xFFFFFFFFu, grow)) {

@@ -54,9 +54,8 @@ def build_bounds(force: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False, lib: Path = LIB_PATH, defines: list[str] | None = None,
           obj_subdir: str = "build") -> Path:
-    """Compile the library (and, with the normal one, the torch binding) if missing or older than its sources."""
-    if lib == LIB_PATH:
-        build_binding(force)
+    """Compile the kernel library if it is missing or older than its sources.  nvcc is all it takes; the torch
+    binding is built by `build_binding`."""
     if not force and not needs_build(lib):
         return lib
     nvcc = _nvcc()
@@ -185,6 +184,6 @@ def compile_program(source: Path, output: Path, extra: list[str] | None = None) 
 if __name__ == "__main__":
     path = build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     print(path)
-    print(BINDING_PATH)
+    print(build_binding(force="--force" in sys.argv))
     print(build_bounds(force="--force" in sys.argv))
     print(build_host(force="--force" in sys.argv))

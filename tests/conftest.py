@@ -19,6 +19,7 @@ def native_lib():
     from kernelcodegen_b200 import build, capi
 
     build.build()
+    build.build_binding()
     return capi.load()
 
 
@@ -38,4 +39,5 @@ def cuda_device():
     from kernelcodegen_b200 import build
 
     build.build()
+    build.build_binding()
     return torch.device("cuda:0")

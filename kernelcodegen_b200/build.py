@@ -91,21 +91,24 @@ BINDING_PATH = PKG_DIR / "_torch_binding.so"
 
 def build_binding(force: bool = False) -> Path:
     """Compile the torch binding of the attention training operators (csrc/torch_binding.cpp) against the
-    installed torch.  Plain C++; it calls the kernel library through addresses it is given at run time."""
-    src, header = CSRC / "torch_binding.cpp", PKG_DIR.parent / "include" / "kcg_capi.h"
-    if not force and BINDING_PATH.exists() and all(p.stat().st_mtime <= BINDING_PATH.stat().st_mtime for p in (src, header)):
-        return BINDING_PATH
+    installed torch.  Plain C++; it calls the kernel library through addresses it is given at run time.
+    Rebuilt when a source is newer, and when torch or Python is not the one it was built with, which it names."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
+    src, header = CSRC / "torch_binding.cpp", PKG_DIR.parent / "include" / "kcg_capi.h"
     cxx = os.environ.get("CXX") or shutil.which("g++") or "g++"
+    built_with = f"torch {torch.__version__} {torch.version.git_version}, Python {sys.version.split()[0]}"
+    if (not force and BINDING_PATH.exists() and built_with.encode() in BINDING_PATH.read_bytes()
+            and all(p.stat().st_mtime <= BINDING_PATH.stat().st_mtime for p in (src, header))):
+        return BINDING_PATH
     cuda_inc = Path(_nvcc()).resolve().parents[1] / "include"
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     tmp = BINDING_PATH.with_suffix(".so.tmp")
     cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DKCG_BUILT_WITH="{built_with}"',
            *(f"-isystem{p}" for p in (*cpp_extension.include_paths(), cuda_inc, sysconfig.get_paths()["include"])),
            str(src), "-o", str(tmp), "-L", str(torch_lib), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            *shared_libstdcxx(cxx)]

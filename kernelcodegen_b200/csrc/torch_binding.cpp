@@ -324,6 +324,7 @@ std::tuple<int, Tensor, Opt, Opt, Opt> qk_norm_rope_backward(const Tensor& dq_ou
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
+  m.attr("built_with") = KCG_BUILT_WITH;
   m.def("bind", &bind);
   // (wrapped: torch's own errors, out of memory among them, keep their Python types)
   m.def("fmha_with_lse", torch::wrap_pybind_function(fmha_with_lse));

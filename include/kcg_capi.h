@@ -236,8 +236,9 @@ kcg_status_t kcg_fmha_fwd_launch(const kcg_fmha_desc* d, const void* Q, const vo
 
 /* Attention forward that also leaves what its gradient needs: O as above and
  * lse[b, h, i] = log sum_j exp(scale * q_i.k_j) over the visible keys (fp32, contiguous [B, H, Sq],
- * natural logarithm; -inf and O = 0 for a query that sees no key).  O must not overlap an input (equal
- * pointers are KCG_BAD_ARGUMENT); the inputs must be finite wherever the tensors have an entry (a masked NaN
+ * natural logarithm; -inf and O = 0 for a query that sees no key).  O and lse must not overlap an input or
+ * one another (KCG_BAD_ARGUMENT wherever the strides show it: equal pointers, views shifted against one another,
+ * heads of one packed buffer); the inputs must be finite wherever the tensors have an entry (a masked NaN
  * still reaches the products it is part of).  No counterpart in the reference, which generates forward
  * kernels only. */
 kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, const void* K, const void* V, void* O,
@@ -248,8 +249,8 @@ kcg_status_t kcg_fmha_fwd_lse_launch(const kcg_attn_desc* d, const void* Q, cons
  *   P_ij = exp(scale q_i.k_j - lse_i), delta_i = dO_i.O_i, dS_ij = P_ij (dO_i.v_j - delta_i),
  *   dV_j = sum_i P_ij dO_i,  dK_j = scale sum_i dS_ij q_i,  dQ_i = scale sum_j dS_ij k_j,
  * the sums of dK and dV over all query heads of the group.  Accumulation in fp32 in a fixed order (the
- * same bits on every call).  The outputs must not overlap one another or an input (equal pointers are
- * KCG_BAD_ARGUMENT); the inputs must be finite, as in the forward call.
+ * same bits on every call).  The outputs must not overlap one another or an input (KCG_BAD_ARGUMENT, as
+ * above); the inputs must be finite, as in the forward call.
  * Workspace: kcg_fmha_bwd_workspace_bytes, not shared by calls that may overlap. */
 size_t kcg_fmha_bwd_workspace_bytes(const kcg_attn_desc* d);
 kcg_status_t kcg_fmha_bwd_launch(const kcg_attn_desc* d, const void* dO, const void* Q, const void* K, const void* V,
@@ -261,8 +262,8 @@ kcg_status_t kcg_fmha_bwd_launch(const kcg_attn_desc* d, const void* dO, const v
  * rotated: (a cos - b sin, b cos + a sin), with the row positions[b, s] of the tables cos, sin (fp32,
  * contiguous [table_rows, R/2]; positions NULL = s).  Computed in fp32, rounded once.  A position
  * outside the tables gives NaN in the rotated entries and code 11 in the status word
- * (kcg_last_device_status); nothing is read there.  An output may be the same view as its input.  No
- * counterpart in the reference. */
+ * (kcg_last_device_status); nothing is read there.  An output may be the same view as its input, the same strides
+ * included, and overlaps nothing else (KCG_BAD_ARGUMENT, as above).  No counterpart in the reference. */
 kcg_status_t kcg_qk_norm_rope_launch(const kcg_rope_desc* d, const void* q, const void* k, const void* q_weight,
                                      const void* k_weight, const void* cos, const void* sin, const void* positions,
                                      void* q_out, void* k_out, void* stream);

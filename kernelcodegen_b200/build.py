@@ -41,7 +41,7 @@ def needs_build(lib: Path = LIB_PATH) -> bool:
     if not lib.exists():
         return True
     t = lib.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + [PKG_DIR.parent / "include" / "kcg_capi.h"]
+    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [PKG_DIR.parent / "include" / "kcg_capi.h"]
     return any(p.stat().st_mtime > t for p in deps if p.exists())
 
 

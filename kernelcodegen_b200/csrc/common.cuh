@@ -9,6 +9,7 @@
 #include <cstdio>
 
 #include "../../include/kcg_capi.h"
+#include "head_view.h"
 
 namespace kcg {
 
@@ -30,23 +31,12 @@ kcg_status_t encode_tmap(CUtensorMap* map, CUtensorMapDataType dt, int rank, con
                          const uint32_t* box,
                          CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
-// Tensor map of a [B, H, S, D] view (strides in elements; the innermost is 1): coordinates
-// (d, row, head, batch), boxes of `rows` rows x 128 bytes, rows past S read as zero.  An extent of one
-// has no stride of its own; it is given one that the encoder accepts.
-struct HeadView {
-  const void* base;
-  int B, H, S, D;
-  int64_t sb, sh, sr;
-};
+// Tensor map of such a view: coordinates (d, row, head, batch), boxes of `rows` rows x 128 bytes, rows past S read
+// as zero.  An extent of one has no stride of its own; it is given one that the encoder accepts.
 kcg_status_t encode_head_view(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const HeadView& v,
                               CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B, int rows = 128);
 // Whether a view can be read through such a map (16-byte rows) or written row by row.
 kcg_status_t check_head_view(const HeadView& v, int elem_bytes);
-// bytes from the first to one past the last element
-inline unsigned long long head_view_extent(const HeadView& v, int elem_bytes) {
-  return (static_cast<unsigned long long>(v.B - 1) * v.sb + static_cast<unsigned long long>(v.H - 1) * v.sh +
-          static_cast<unsigned long long>(v.S - 1) * v.sr + v.D) * elem_bytes;
-}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

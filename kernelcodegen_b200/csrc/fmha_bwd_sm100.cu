@@ -850,9 +850,11 @@ kcg_status_t fmha_bwd_launch_impl(const kcg_attn_desc* d, const void* dO, const 
   const BwdPlan n = plan_bwd(d);
   if (!ws || ws_bytes < n.bytes() || !aligned16(ws)) return KCG_BAD_WORKSPACE;
   // an output over an input or another output: it would be written while other CTAs still read it
-  for (const void* x : {dO, Q, K, V, O})
-    if (x == dQ || x == dK || x == dV) return KCG_BAD_ARGUMENT;
-  if (dQ == dK || dQ == dV || dK == dV) return KCG_BAD_ARGUMENT;
+  const HeadRegion regions[9] = {{vdq, 2}, {vdk, 2}, {vdv, 2}, {vdo, 2}, {vq, 2}, {vk, 2}, {vv, 2}, {vo, 2},
+                                 {HeadView{lse, d->B, d->H, d->Sq, 1, static_cast<int64_t>(d->H) * d->Sq, d->Sq, 1}, 4}};
+  for (int out = 0; out < 3; ++out)
+    for (int i = out + 1; i < 9; ++i)
+      if (views_overlap(regions[out], regions[i])) return KCG_BAD_ARGUMENT;
   const long long ctas = n.kv_items * n.kv_split + n.q_items * n.q_split;
   if (ctas > 0x7FFFFFFFll || static_cast<long long>(d->H / d->Hkv) * n.n_qt > 0x3FFFFFFFll) return KCG_BAD_SHAPE;
   CUtensorMap tq, tk, tv, tdo;

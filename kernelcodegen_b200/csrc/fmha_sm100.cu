@@ -773,7 +773,11 @@ kcg_status_t fmha_lse_launch_impl(const kcg_attn_desc* d, const void* Q, const v
   const HeadView vo{O, d->B, d->H, d->Sq, d->D, d->o[0], d->o[1], d->o[2]};
   for (const HeadView* v : {&vq, &vk, &vv, &vo})
     if ((st = check_head_view(*v, 2)) != KCG_OK) return st;
-  if (O == Q || O == K || O == V) return KCG_BAD_ARGUMENT;   // written while other CTAs still read it
+  // written while other CTAs still read them, or one over the other
+  const HeadRegion out(vo, 2), stat(HeadView{lse, d->B, d->H, d->Sq, 1, static_cast<int64_t>(d->H) * d->Sq, d->Sq, 1}, 4);
+  for (const HeadView* v : {&vq, &vk, &vv})
+    if (views_overlap(out, HeadRegion(*v, 2)) || views_overlap(stat, HeadRegion(*v, 2))) return KCG_BAD_ARGUMENT;
+  if (views_overlap(out, stat)) return KCG_BAD_ARGUMENT;
   CUtensorMap tq, tk, tv;
   if ((st = encode_head_view(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vq)) != KCG_OK) return st;
   if ((st = encode_head_view(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, vk)) != KCG_OK) return st;

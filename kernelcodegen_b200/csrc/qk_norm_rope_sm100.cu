@@ -717,6 +717,25 @@ kcg_status_t fill(const kcg_rope_desc* d, const void* const (&x)[2], const int64
       if (k == 2) p.y_extent[t] = head_view_extent(v, es);
     }
   }
+  // An output is written while other groups of lanes still read: it may be the very view that its own rows are read
+  // from (a row is read before it is written, by the same lanes), and may overlap nothing else.
+  auto view = [&](const void* at, const long long (&s)[3], int t) { return HeadView{at, d->B, p.heads[t], d->S, d->D, s[0], s[1], s[2]}; };
+  for (int t = 0; t < 2; ++t) {
+    if (!p.heads[t]) continue;
+    const HeadRegion out(view(p.y[t], p.ys[t], t), es);
+    for (int u = 0; u < 2; ++u) {
+      if (!p.heads[u]) continue;
+      const void* in[2] = {p.x[u], p.dy[u]};
+      const long long(*st[2])[3] = {&p.xs[u], &p.ds[u]};
+      for (int k = 0; k < 2; ++k) {
+        if (!in[k]) continue;
+        const long long(&s)[3] = *st[k];
+        const bool same = u == t && in[k] == p.y[t] && s[0] == p.ys[t][0] && s[1] == p.ys[t][1] && s[2] == p.ys[t][2];
+        if (!same && views_overlap(out, HeadRegion(view(in[k], s, u), es))) return KCG_BAD_ARGUMENT;
+      }
+    }
+    if (t && p.heads[0] && views_overlap(out, HeadRegion(view(p.y[0], p.ys[0], 0), es))) return KCG_BAD_ARGUMENT;
+  }
   p.w_f32 = d->dtype_w == KCG_F32;
   p.cs = static_cast<const float*>(cs);
   p.sn = static_cast<const float*>(sn);

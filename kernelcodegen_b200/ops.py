@@ -264,8 +264,8 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
     cos, sin: float32 [positions, R / 2] tables; pairs are (i, i + R/2), or (2i, 2i + 1) if `interleaved`.
     positions: int32 or int64 [S] or [B, S], None for 0..S-1; a position outside the tables makes the
     row's rotated entries NaN and sets `last_device_status()` to 11.
-    The outputs are contiguous [B, heads, S, D] unless q_out / k_out is given (a slice of a key cache, or
-    the input itself)."""
+    The outputs are contiguous [B, heads, S, D] unless q_out / k_out is given: a slice of a key cache, or
+    the input itself (the same view), but nothing that overlaps in another way."""
     st, q_out, k_out = (_native or _binding()).qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
                                                             q_out, k_out)
     if st:
@@ -282,7 +282,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], 
     """(dq, dk, dq_weight, dk_weight) of `qk_norm_rope` for the gradients of its outputs and the inputs
     it was called with.  The weights' gradients are float32 [D], summed over batch, heads and tokens in a
     fixed order (None for a weight that is None).  dq and dk are contiguous unless given; they may be
-    dq_out and dk_out themselves."""
+    dq_out and dk_out, or q and k, themselves (the same views)."""
     st, dq, dk, dqw, dkw = (_native or _binding()).qk_norm_rope_backward(dq_out, dk_out, q, k, cos, sin, q_weight, k_weight,
                                                                          positions, eps, interleaved, dq, dk)
     if st:

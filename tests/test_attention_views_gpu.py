@@ -1,0 +1,71 @@
+"""Views that the attention training operators take side by side in one buffer."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def make(shape, seed, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dtype).cuda()
+
+
+def tables(rows, R):
+    angle = torch.arange(rows, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64) / R)
+    return angle.cos().float().cuda(), angle.sin().float().cuda()
+
+
+@pytest.mark.parametrize("layout", ["heads of a token in a row", "q, k, v of a head in a row", "tensors in a row", "batches interleaved"])
+def test_everything_in_one_buffer(cuda_device, layout):
+    """Inputs, output and gradients interleaved in one allocation: the bits of separate tensors."""
+    from kernelcodegen_b200 import ops
+
+    B, H, S, D = 2, 3, 70, 64
+    n = 8                                   # q, k, v, out, dout, dq, dk, dv
+    if layout == "heads of a token in a row":
+        views = torch.zeros((B, S, n, H, D), device="cuda", dtype=torch.bfloat16).permute(2, 0, 3, 1, 4)
+    elif layout == "q, k, v of a head in a row":
+        views = torch.zeros((B, S, H, n, D), device="cuda", dtype=torch.bfloat16).permute(3, 0, 2, 1, 4)
+    elif layout == "tensors in a row":
+        views = torch.zeros((n, B, H, S, D), device="cuda", dtype=torch.bfloat16)
+    else:
+        views = torch.zeros((B, n, H, S, D), device="cuda", dtype=torch.bfloat16).transpose(0, 1)
+    q, k, v, out, dout, dq, dk, dv = views.unbind(0)
+    flat = [make((B, H, S, D), s) for s in range(4)]
+    for view, t in zip((q, k, v, dout), flat):
+        view.copy_(t)
+    _, lse = ops.fmha_with_lse(q, k, v, scale=0.1, causal=True, out=out)
+    ops.fmha_backward(dout, q, k, v, out, lse, scale=0.1, causal=True, dq=dq, dk=dk, dv=dv)
+    out2, lse2 = ops.fmha_with_lse(*flat[:3], scale=0.1, causal=True)
+    grads = ops.fmha_backward(flat[3], *flat[:3], out2, lse2, scale=0.1, causal=True)
+    for a, b in zip((out, lse, dq, dk, dv), (out2, lse2, *grads)):
+        assert torch.equal(a, b)
+    for view, t in zip((q, k, v, dout), flat):
+        assert torch.equal(view, t)
+    cos, sin = tables(S, D)
+    want = ops.qk_norm_rope(flat[0], flat[1], cos, sin)
+    ops.qk_norm_rope(q, k, cos, sin, q_out=dq, k_out=dk)
+    assert torch.equal(dq, want[0]) and torch.equal(dk, want[1])
+    grads = ops.qk_norm_rope_backward(flat[3], flat[2], flat[0], flat[1], cos, sin)
+    ops.qk_norm_rope_backward(dout, v, q, k, cos, sin, dq=dq, dk=dk)
+    assert torch.equal(dq, grads[0]) and torch.equal(dk, grads[1])
+    ops.qk_norm_rope_backward(dout, v, q, k, cos, sin, dq=dout, dk=v)          # over the gradients that came in
+    assert torch.equal(dout, grads[0]) and torch.equal(v, grads[1])
+    assert torch.equal(q, flat[0]) and torch.equal(k, flat[1])
+    assert ops.last_device_status() == 0
+
+
+def test_one_place_of_a_cache_to_another(cuda_device):
+    """A key read from one place of a cache and written to another, and over itself."""
+    from kernelcodegen_b200 import ops
+
+    cache = make((2, 3, 20, 64), 1)
+    keep, q = cache.clone(), make((2, 4, 1, 64), 2)
+    cos, sin = tables(20, 64)
+    at = torch.tensor([7], device="cuda")
+    _, want = ops.qk_norm_rope(q, keep[:, :, 4:5].contiguous(), cos, sin, positions=at)
+    for to in (5, 3, 19, 4):
+        ops.qk_norm_rope(q, cache[:, :, 4:5], cos, sin, positions=at, k_out=cache[:, :, to:to + 1])
+        assert torch.equal(cache[:, :, to:to + 1], want)
+    rest = [i for i in range(20) if i not in (3, 4, 5, 19)]
+    assert torch.equal(cache[:, :, rest], keep[:, :, rest])

@@ -85,6 +85,14 @@ Tensor contiguous(at::IntArrayRef shape, at::ScalarType dtype, at::Device dev) {
   return at::detail::empty_strided_cuda(shape, at::IntArrayRef(strides.data(), shape.size()), dtype, dev);
 }
 
+// The same, of a tensor that has to have memory of its own for every entry: what autograd hands out for a broadcast has not.
+Strides own_view(const char* name, const Tensor& t, const Shape& shape, at::ScalarType dtype, at::Device dev) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0)
+      bad_value(std::string(name) + " is an expanded tensor (stride 0 in dimension " + std::to_string(i) + "): call .contiguous() on it first");
+  return view(name, t, shape, dtype, dev);
+}
+
 // An output view: the one given, checked, or a new contiguous tensor.
 Strides output(const char* name, const Opt& given, const Shape& shape, at::ScalarType dtype, at::Device dev, Tensor& out) {
   out = given ? *given : contiguous(shape, dtype, dev);
@@ -128,9 +136,9 @@ Attn attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, 
   a.d.dtype = KCG_BF16;
   a.d.causal = causal;
   a.d.scale = static_cast<float>(scale);
-  put(a.d.q, view("Q", q, a.q, bf16, a.dev));
-  put(a.d.k, view("K", k, a.k, bf16, a.dev));
-  put(a.d.v, view("V", v, a.k, bf16, a.dev));
+  put(a.d.q, own_view("Q", q, a.q, bf16, a.dev));
+  put(a.d.k, own_view("K", k, a.k, bf16, a.dev));
+  put(a.d.v, own_view("V", v, a.k, bf16, a.dev));
   a.empty = q.numel() == 0 || k.numel() == 0;
   return a;
 }
@@ -164,8 +172,8 @@ std::tuple<int, Tensor, Tensor, Tensor> fmha_backward(const Tensor& dout, const 
                                                       const Opt& dq_, const Opt& dk_, const Opt& dv_) {
   Attn a = attention(q, k, v, scale, causal);
   const auto bf16 = at::kBFloat16;
-  put(a.d.d_o, view("dout", dout, a.q, bf16, a.dev));
-  put(a.d.o, view("out", out, a.q, bf16, a.dev));
+  put(a.d.d_o, own_view("dout", dout, a.q, bf16, a.dev));
+  put(a.d.o, own_view("out", out, a.q, bf16, a.dev));
   if (lse.dim() != 3 || lse.size(0) != a.q[0] || lse.size(1) != a.q[1] || lse.size(2) != a.q[2] ||
       lse.scalar_type() != at::kFloat || !lse.is_contiguous())
     bad_value("lse must be the contiguous float32 [B,H,Sq] tensor of fmha_with_lse");

@@ -224,10 +224,11 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
                   out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """`fmha` for a forward pass that will be differentiated: (O, lse), lse[b, h, i] = log sum_j
     exp(scale q_i.k_j) in float32 [B, H, Sq] (-inf, and O = 0, for a query that sees no key).
-    bfloat16 [B, H, S, D] views with any strides that are multiples of 16 bytes and stride 1 in the
-    last dimension (heads of a packed projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may
-    have fewer heads, Hkv | H, and query head h then reads head h // (H // Hkv).  D is 64 or 128.  Any other
-    extent may be zero: with no keys O = 0 and lse = -inf.
+    bfloat16 [B, H, S, D] views with any strides that are positive multiples of 16 bytes (an expanded
+    tensor, stride 0, wants .contiguous()) and stride 1 in the last dimension (heads of a packed
+    projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may have fewer heads, Hkv | H, and query
+    head h then reads head h // (H // Hkv).  D is 64 or 128.  Any other extent may be zero: with no keys
+    O = 0 and lse = -inf.
     O is contiguous unless `out` is given (not over an input).  All entries must be finite, those that no
     query sees too: they take part in the products with weight zero."""
     st, out, lse = (_native or _binding()).fmha_with_lse(q, k, v, scale, causal, out)
@@ -241,9 +242,9 @@ def fmha_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
                   dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None
                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dQ, dK, dV) of `fmha_with_lse`, from the gradient of its O and the `out` and `lse` it returned
-    (call with the same scale and causal).  Views as there; the gradients are contiguous unless dq, dk or
-    dv is given, e.g. as the heads of a packed gradient.  Outputs must not overlap one another or an
-    input.  The same bits on every call: nothing is added up in an order that can change.  Zero where an
+    (call with the same scale and causal).  Views as there (the expanded dout of a broadcast loss, such as
+    out.sum(), wants .contiguous()); the gradients are contiguous unless dq, dk or dv is given, e.g. as the
+    heads of a packed gradient.  Outputs must not overlap one another or an input.  The same bits on every call: nothing is added up in an order that can change.  Zero where an
     extent of zero leaves nothing to sum."""
     st, dq, dk, dv = (_native or _binding()).fmha_backward(dout, q, k, v, out, lse, scale, causal, dq, dk, dv)
     if st:

@@ -1,4 +1,5 @@
-"""Views that the attention training operators take side by side in one buffer."""
+"""Views that the attention training operators take side by side in one buffer, and those that they refuse with a
+reason: expanded ones (stride 0), which autograd hands out."""
 import pytest
 import torch
 
@@ -69,3 +70,29 @@ def test_one_place_of_a_cache_to_another(cuda_device):
         assert torch.equal(cache[:, :, to:to + 1], want)
     rest = [i for i in range(20) if i not in (3, 4, 5, 19)]
     assert torch.equal(cache[:, :, rest], keep[:, :, rest])
+
+
+def test_expanded_tensors_are_refused_by_name(cuda_device):
+    from kernelcodegen_b200 import ops
+
+    q, k = make((2, 4, 64, 64), 1), make((2, 2, 64, 64), 2)
+    out, lse = ops.fmha_with_lse(q, k, k)
+    row = make((2, 4, 1, 64), 3)
+    with pytest.raises(ValueError, match="dout.*stride 0.*contiguous"):
+        ops.fmha_backward(row.expand(q.shape), q, k, k, out, lse)
+    with pytest.raises(ValueError, match="dout.*stride 0.*contiguous"):         # what out.sum().backward() hands out
+        ops.fmha_backward(torch.ones((), device="cuda", dtype=torch.bfloat16).expand(q.shape), q, k, k, out, lse)
+    with pytest.raises(ValueError, match="K.*stride 0.*contiguous"):
+        ops.fmha_with_lse(q, k[:, :1].expand(2, 4, 64, 64), k.repeat(1, 2, 1, 1))
+    with pytest.raises(ValueError, match="V.*stride 0.*contiguous"):
+        ops.fmha_with_lse(q, k, k[:1].expand(2, 2, 64, 64))
+    # an extent of one has no stride to speak of
+    one = make((1, 1, 1, 64), 4)
+    a, b = ops.fmha_with_lse(one.as_strided((1, 1, 1, 64), (0, 0, 0, 1)), one, one)
+    assert torch.equal(a, one) and torch.isfinite(b).all()
+    # norm and rotation read expanded rows
+    cos, sin = tables(64, 64)
+    y, _ = ops.qk_norm_rope(row.expand(q.shape), None, cos, sin)
+    assert torch.equal(y, ops.qk_norm_rope(row.expand(q.shape).contiguous(), None, cos, sin)[0])
+    dy, _, _, _ = ops.qk_norm_rope_backward(row.expand(q.shape), None, q, None, cos, sin)
+    assert torch.equal(dy, ops.qk_norm_rope_backward(row.expand(q.shape).contiguous(), None, q, None, cos, sin)[0])

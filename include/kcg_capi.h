@@ -379,7 +379,7 @@ void kcg_set_spin_limit(uint32_t iterations);
 
 /* Bounds-checking build.  The library can be built a second time with -DKCG_DEBUG_BOUNDS
  * (libkcg_b200_bounds.so; kernelcodegen_b200.build.build_bounds()).  In that build every global
- * store of a result and every access to the shared-K scratch is checked against the byte extent
+ * store of a result and every access to scratch memory is checked against the byte extent
  * of its buffer, and the launch code checks every tensor-map coordinate it will issue for the
  * 16-byte rule; a failed device-side check records code 10 in the status word
  * (kcg_last_device_status) and the offending offset / extent (kcg_debug_bounds_detail), SKIPS the

@@ -81,6 +81,7 @@ struct BwdParams {
   int* status;
   uint32_t spin;
   unsigned long long dq_extent, dk_extent, dv_extent;   // bounds-checking build
+  unsigned long long stat_extent, part_q_extent, part_kv_extent;
   unsigned long long* bounds_detail;
 };
 
@@ -337,9 +338,12 @@ __device__ __forceinline__ void run_item(const CUtensorMap* tmA0, const CUtensor
           if (i == 0) griddep_wait();
           const size_t at = (static_cast<size_t>(w.b) * p.H + py.h) * p.sq_pad + static_cast<size_t>(py.t) * BN;
           const uint32_t bar = b_tfull + 8 * tr.stage, to = s_stat + tr.stage * Cfg::STAT_BYTES;
-          mbar_expect_tx(bar, Cfg::STAT_BYTES);
-          bulk_load(to, p.nlse + at, BN * 4, bar);
-          bulk_load(to + BN * 4, p.ndelta + at, BN * 4, bar);
+          const bool inside = bounds_ok(at * 4, BN * 4, p.stat_extent, p.status, p.bounds_detail);
+          mbar_expect_tx(bar, inside ? Cfg::STAT_BYTES : 0);
+          if (inside) {
+            bulk_load(to, p.nlse + at, BN * 4, bar);
+            bulk_load(to + BN * 4, p.ndelta + at, BN * 4, bar);
+          }
           tr.next();
         }
         step_place(py);
@@ -488,8 +492,10 @@ __device__ __forceinline__ void run_item(const CUtensorMap* tmA0, const CUtensor
     if (!KV && n_it > 0) {
       griddep_wait();
       const size_t at = (static_cast<size_t>(w.b) * p.H + w.head) * p.sq_pad + row;   // row < sq_pad
-      nl = p.nlse[at];
-      nd = p.ndelta[at];
+      if (bounds_ok(at * 4, 4, p.stat_extent, p.status, p.bounds_detail)) {
+        nl = p.nlse[at];
+        nd = p.ndelta[at];
+      }
     }
     int t = n_it > 0 ? w.it0 % w.n_tiles : 0;
     for (int i = 0; i < n_it; ++i) {
@@ -606,10 +612,12 @@ __device__ __forceinline__ void run_item(const CUtensorMap* tmA0, const CUtensor
         float* part = KV ? (is_v ? p.part_v : p.part_k) : p.part_q;
         const size_t items = static_cast<size_t>(KV ? p.bhkv : p.bh) * (KV ? p.n_kt : p.n_qt);
         const size_t item = (static_cast<size_t>(w.b) * (KV ? p.Hkv : p.H) + w.head) * (KV ? p.n_kt : p.n_qt) + w.row0 / BT;
-        float4* dst = reinterpret_cast<float4*>(part) + ((w.piece * items + item) * (D / 4) + col / 4) * BT + r;
+        const size_t at = ((w.piece * items + item) * (D / 4) + col / 4) * BT + r;
+        float4* dst = reinterpret_cast<float4*>(part) + at;
+        if (bounds_ok(at * 16, (7 * BT + 1) * 16, KV ? p.part_kv_extent : p.part_q_extent, p.status, p.bounds_detail))
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          dst[k * BT] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
+          for (int k = 0; k < 8; ++k)
+            dst[k * BT] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
       }
     }
     if (whole) {
@@ -669,6 +677,9 @@ struct StatParams {
   long long o_sb, o_sh, o_sr, g_sb, g_sh, g_sr;
   int H, Sq, sq_pad;
   long long rows;         // B * H * sq_pad
+  int* status;            // bounds-checking build
+  unsigned long long extent;
+  unsigned long long* bounds_detail;
 };
 
 template <int D>
@@ -698,7 +709,7 @@ __global__ void __launch_bounds__(256) fmha_bwd_stat_kernel(const StatParams p) 
     }
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (sub == 0) {
+    if (sub == 0 && bounds_ok(at * 4, 4, p.extent, p.status, p.bounds_detail)) {
       p.nlse[at] = nl;
       p.ndelta[at] = -sum;
     }
@@ -718,6 +729,7 @@ __global__ void __launch_bounds__(256) fmha_bwd_sum_kernel(const __grid_constant
   const long long sb = which == 2 ? p.q_sb : which ? p.v_sb : p.k_sb, sh = which == 2 ? p.q_sh : which ? p.v_sh : p.k_sh,
                   sr = which == 2 ? p.q_sr : which ? p.v_sr : p.k_sr;
   const unsigned long long extent = which == 2 ? p.dq_extent : which ? p.dv_extent : p.dk_extent;
+  const unsigned long long part_extent = which == 2 ? p.part_q_extent : p.part_kv_extent;
   const int heads = which == 2 ? p.H : p.Hkv, rows = which == 2 ? p.Sq : p.Skv, tiles = which == 2 ? p.n_qt : p.n_kt;
   const long long items = static_cast<long long>(which == 2 ? p.bh : p.bhkv) * tiles, piece = items * (D / 4) * BT;
   const float f = which == 1 ? 1.f : p.scale;
@@ -727,10 +739,12 @@ __global__ void __launch_bounds__(256) fmha_bwd_sum_kernel(const __grid_constant
     const long long item = i / (D / 8);
     const int col = static_cast<int>(i % (D / 8)) * 8, row = static_cast<int>(item % tiles) * BT + r;
     const long long bh = item / tiles;
-    const float4* src = reinterpret_cast<const float4*>(part) + (item * (D / 4) + col / 4) * BT + r;
+    const long long first = (item * (D / 4) + col / 4) * BT + r;
+    const float4* src = reinterpret_cast<const float4*>(part) + first;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
 #pragma unroll 4
     for (int s = 0; s < split; ++s) {
+      if (!bounds_ok((first + s * piece) * 16, (BT + 1) * 16, part_extent, p.status, p.bounds_detail)) continue;
       const float4 x = src[s * piece], y = src[s * piece + BT];
       a = make_float4(a.x + x.x, a.y + x.y, a.z + x.z, a.w + x.w);
       b = make_float4(b.x + y.x, b.y + y.y, b.z + y.z, b.w + y.w);
@@ -908,11 +922,18 @@ kcg_status_t fmha_bwd_launch_impl(const kcg_attn_desc* d, const void* dO, const 
   p.dq_extent = head_view_extent(vdq, 2);
   p.dk_extent = head_view_extent(vdk, 2);
   p.dv_extent = head_view_extent(vdv, 2);
+  p.stat_extent = n.stat_floats * 4;
+  p.part_q_extent = n.part_q * 4;
+  p.part_kv_extent = n.part_kv * 4;
   if (const unsigned long long cap = debug_extent_limit())
-    for (unsigned long long* e : {&p.dq_extent, &p.dk_extent, &p.dv_extent}) *e = *e < cap ? *e : cap;
+    for (unsigned long long* e : {&p.dq_extent, &p.dk_extent, &p.dv_extent, &p.stat_extent, &p.part_q_extent, &p.part_kv_extent})
+      *e = *e < cap ? *e : cap;
   p.bounds_detail = nullptr;
   debug_bounds_detail_ptr(&p.bounds_detail);
   if ((st = device_status_ptr(&p.status)) != KCG_OK) return st;
+  s.status = p.status;
+  s.extent = p.stat_extent;
+  s.bounds_detail = p.bounds_detail;
   const uint32_t spin = g_spin_limit.load();
   p.spin = spin ? spin : KCG_SPIN_LIMIT;
   if (d->D == 64) return launch_bwd<64>(tq, tk, tv, tdo, p, s, ctas, stream);

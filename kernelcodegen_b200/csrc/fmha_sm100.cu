@@ -52,6 +52,7 @@ struct FmhaParams {
   int Sq, Skv;
   long long o_sb, o_sh, o_sr;  // strides of O in elements
   float* lse;        // [B, H, Sq] log-sum-exp of every row's scaled scores (LSE instantiations)
+  unsigned long long lse_extent;  // bounds-checking build
   int causal;
   int out_bf16;
   float scale_log2;  // scale * log2(e)
@@ -511,12 +512,16 @@ fmha_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       }
     }
     const size_t off = static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(h) * p.o_sh + static_cast<size_t>(row) * p.o_sr;
+    if (LSE && ok && row < p.Sq) {
+      const size_t at = static_cast<size_t>(bh) * p.Sq + row;
+      if (bounds_ok(at * 4, 4, p.lse_extent, p.status, p.bounds_detail))
+        p.lse[at] = l <= 1e-30f ? -INFINITY : (m * c + __log2f(l)) * 0.6931471805599453f;
+    }
     if (ok && row < p.Sq &&
         bounds_ok(off * (p.out_bf16 ? 2 : 4), static_cast<unsigned long long>(D) * (p.out_bf16 ? 2 : 4), p.o_extent,
                   p.status, p.bounds_detail)) {
       // a row with no visible key sums to < 2^-100
       const float inv = (LSE ? l <= 1e-30f : !(l > 1e-30f)) ? 0.f : 1.f / l;
-      if (LSE) p.lse[static_cast<size_t>(bh) * p.Sq + row] = l <= 1e-30f ? -INFINITY : (m * c + __log2f(l)) * 0.6931471805599453f;
       if (p.out_bf16) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.O) + off);
 #pragma unroll
@@ -725,6 +730,7 @@ kcg_status_t fmha_launch_impl(const kcg_fmha_desc* d, const void* Q, const void*
   FmhaParams p;
   p.O = O;
   p.lse = nullptr;
+  p.lse_extent = 0;
   p.H = d->H;
   p.group = 1;
   p.o_sb = static_cast<long long>(d->H) * d->Sq * d->D;
@@ -796,7 +802,9 @@ kcg_status_t fmha_lse_launch_impl(const kcg_attn_desc* d, const void* Q, const v
   p.out_bf16 = 1;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.o_extent = head_view_extent(HeadView{O, d->B, d->H, d->Sq, d->D, p.o_sb, p.o_sh, p.o_sr}, 2);
-  if (const unsigned long long cap = debug_extent_limit()) p.o_extent = p.o_extent < cap ? p.o_extent : cap;
+  p.lse_extent = 4ull * d->B * d->H * d->Sq;
+  if (const unsigned long long cap = debug_extent_limit())
+    for (unsigned long long* e : {&p.o_extent, &p.lse_extent}) *e = *e < cap ? *e : cap;
   p.bounds_detail = nullptr;
   debug_bounds_detail_ptr(&p.bounds_detail);
   if ((st = device_status_ptr(&p.status)) != KCG_OK) return st;

@@ -46,7 +46,7 @@ struct RopeParams {
   int ctas[2];                    // backward: CTAs of each tensor
   float* part;                    // backward: [ctas][D] partial weight gradients; null when none is wanted
   int* status;
-  unsigned long long y_extent[2]; // bounds-checking build
+  unsigned long long y_extent[2], part_extent, dw_extent; // bounds-checking build
   unsigned long long* bounds_detail;
 };
 
@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_vec_kernel(const __grid_co
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < RN_THREADS / 32; ++k) sum += red[k][i];
-      p.part[static_cast<long long>(blockIdx.x) * p.D + i] = sum;
+      const long long at = static_cast<long long>(blockIdx.x) * p.D + i;
+      if (bounds_ok(at * 4, 4, p.part_extent, p.status, p.bounds_detail)) p.part[at] = sum;
     }
   }
 }
@@ -533,34 +534,37 @@ __global__ void __launch_bounds__(RN_THREADS, 2) rope_pair_kernel(const __grid_c
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < RN_THREADS / 32; ++k) sum += red[k][i];
-      p.part[static_cast<long long>(blockIdx.x) * p.D + i] = sum;
+      const long long at = static_cast<long long>(blockIdx.x) * p.D + i;
+      if (bounds_ok(at * 4, 4, p.part_extent, p.status, p.bounds_detail)) p.part[at] = sum;
     }
   }
 }
 
 // dw[i] = sum of the CTAs' partial sums, in a fixed order (zero where there are none: no key heads): 32 columns per
 // CTA, a warp per 32nd row.  Its launch overlaps the kernel before it.
-__global__ void __launch_bounds__(1024) rope_weight_sum_kernel(const float* part, int count0, int count1, int D, float* dw0,
-                                                               float* dw1) {
+__global__ void __launch_bounds__(1024) rope_weight_sum_kernel(const __grid_constant__ RopeParams p, float* dw0, float* dw1) {
   __shared__ float red[32][33];
   float* dw = blockIdx.y ? dw1 : dw0;
   if (!dw) return;
   const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane;
-  const int n = blockIdx.y ? count1 : count0;
-  const float* rows = part + (blockIdx.y ? static_cast<long long>(count0) * D : 0) + col;
+  const int col = blockIdx.x * 32 + lane, D = p.D;
+  const int n = p.ctas[blockIdx.y];
+  const long long first = (blockIdx.y ? static_cast<long long>(p.ctas[0]) * D : 0) + col;
   griddep_wait();
   float sum = 0.f;
   if (col < D) {
 #pragma unroll 4
-    for (int i = sub; i < n; i += 32) sum += rows[static_cast<long long>(i) * D];
+    for (int i = sub; i < n; i += 32) {
+      const long long at = first + static_cast<long long>(i) * D;
+      if (bounds_ok(at * 4, 4, p.part_extent, p.status, p.bounds_detail)) sum += p.part[at];
+    }
   }
   red[sub][lane] = sum;
   __syncthreads();
   if (sub == 0 && col < D) {
 #pragma unroll
     for (int k = 1; k < 32; ++k) sum += red[k][lane];
-    dw[col] = sum;
+    if (bounds_ok(col * 4, 4, p.dw_extent, p.status, p.bounds_detail)) dw[col] = sum;
   }
 }
 
@@ -751,8 +755,10 @@ kcg_status_t fill(const kcg_rope_desc* d, const void* const (&x)[2], const int64
   p.inv_d = 1.f / static_cast<float>(d->D);
   p.part = nullptr;
   p.ctas[0] = p.ctas[1] = 0;
+  p.part_extent = qk_norm_rope_bwd_workspace_impl(d);
+  p.dw_extent = 4ull * d->D;
   if (const unsigned long long cap = debug_extent_limit())
-    for (unsigned long long& e : p.y_extent) e = e < cap ? e : cap;
+    for (unsigned long long* e : {&p.y_extent[0], &p.y_extent[1], &p.part_extent, &p.dw_extent}) *e = *e < cap ? *e : cap;
   p.bounds_detail = nullptr;
   debug_bounds_detail_ptr(&p.bounds_detail);
   return device_status_ptr(&p.status);
@@ -811,8 +817,7 @@ kcg_status_t qk_norm_rope_bwd_impl(const kcg_rope_desc* d, const void* dq_out, c
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  KCG_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_weight_sum_kernel, static_cast<const float*>(p.part), p.ctas[0], p.ctas[1],
-                                  static_cast<int>(d->D), dwq, dwk));
+  KCG_CUDA_TRY(cudaLaunchKernelEx(&cfg, rope_weight_sum_kernel, p, dwq, dwk));
   g_launches.fetch_add(1);
   return KCG_OK;
 }

@@ -229,8 +229,11 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
     projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may have fewer heads, Hkv | H, and query
     head h then reads head h // (H // Hkv).  D is 64 or 128.  Any other extent may be zero: with no keys
     O = 0 and lse = -inf.
-    O is contiguous unless `out` is given (not over an input).  All entries must be finite, those that no
-    query sees too: they take part in the products with weight zero."""
+    causal: query i sees the keys j <= i + Skv - Sq.  O is contiguous unless `out` is given (not over an
+    input).  All entries must be finite, those that no query sees too: they take part in the products with
+    weight zero; a visible score that overflows float32 makes its row's O and lse NaN.
+    Scores, maxima and sums are float32 (2^x good to 3e-6); P is rounded to bfloat16 for its product with V.
+    No autograd history is recorded: pair it with `fmha_backward` in a `torch.autograd.Function`."""
     st, out, lse = (_native or _binding()).fmha_with_lse(q, k, v, scale, causal, out)
     if st:
         capi.check(st, "kcg_fmha_fwd_lse_launch")
@@ -244,8 +247,9 @@ def fmha_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     """(dQ, dK, dV) of `fmha_with_lse`, from the gradient of its O and the `out` and `lse` it returned
     (call with the same scale and causal).  Views as there (the expanded dout of a broadcast loss, such as
     out.sum(), wants .contiguous()); the gradients are contiguous unless dq, dk or dv is given, e.g. as the
-    heads of a packed gradient.  Outputs must not overlap one another or an input.  The same bits on every call: nothing is added up in an order that can change.  Zero where an
-    extent of zero leaves nothing to sum."""
+    heads of a packed gradient.  Outputs must not overlap one another or an input.  The same bits on every
+    call: nothing is added up in an order that can change.  Zero where an extent of zero leaves nothing to
+    sum.  Sums are float32; P and dS are rounded to bfloat16 for their products."""
     st, dq, dk, dv = (_native or _binding()).fmha_backward(dout, q, k, v, out, lse, scale, causal, dq, dk, dv)
     if st:
         capi.check(st, "kcg_fmha_bwd_launch")
@@ -266,7 +270,9 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, 
     positions: int32 or int64 [S] or [B, S], None for 0..S-1; a position outside the tables makes the
     row's rotated entries NaN and sets `last_device_status()` to 11.
     The outputs are contiguous [B, heads, S, D] unless q_out / k_out is given: a slice of a key cache, or
-    the input itself (the same view), but nothing that overlaps in another way."""
+    the input itself (the same view), but nothing that overlaps in another way.  The arithmetic is float32,
+    the squares' sum included, rounded once.  No autograd history is recorded: pair it with
+    `qk_norm_rope_backward` in a `torch.autograd.Function`."""
     st, q_out, k_out = (_native or _binding()).qk_norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
                                                             q_out, k_out)
     if st:

@@ -1,5 +1,6 @@
-"""B200 (sm_100a) kernels for the two operators KernelCodeGen generates: fused matmul+ReLU
-and FMHA, behind a C-ABI (`include/kcg_capi.h`)."""
+"""B200 (sm_100a) kernels for the operators KernelCodeGen generates (fused matmul+ReLU and FMHA), the standalone
+softmax, transpose and batched product, and attention for training with the norm and rotation of its queries and
+keys, behind a C-ABI (`include/kcg_capi.h`)."""
 from . import capi  # noqa: F401
 
 __all__ = ["capi", "ops"]

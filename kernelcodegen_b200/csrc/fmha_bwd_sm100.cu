@@ -781,9 +781,11 @@ struct BwdPlan {
 };
 
 // An item is cut where it alone would outlast an equal share of the whole launch on every CTA that the SMs
-// hold (costs in products: 4 a tile in a kv item, 3 in a q item), into pieces of such a share, but of 512
-// rows of its stream or more (a CTA's start and end take as long as about two 128-row tiles).  The SM
-// count is the B200's, so that the workspace query needs no device.
+// hold (costs in products: 4 a tile in a kv item, 3 in a q item), into pieces of such a share, but of about 512
+// rows of the longest item's stream (a CTA's start and end take as long as about two 128-row tiles); the count is
+// rounded to the nearest, so that 768 rows make two pieces of 384.  All items of a kind are cut alike: under the mask
+// the short ones have shorter pieces, down to none, whose CTAs write zeros.  The SM count is the B200's, so that the
+// workspace query needs no device.
 BwdPlan plan_bwd(const kcg_attn_desc* d) {
   BwdPlan n;
   const long long sq_pad = static_cast<long long>(stat_pad(d->Sq));

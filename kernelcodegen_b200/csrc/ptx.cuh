@@ -24,7 +24,7 @@ enum DeviceStatus : int {
   DEV_TIMEOUT_PEER = 9,       // a rank's completion flag did not arrive in time (kcg_peer_wait_launch)
   DEV_BOUNDS = 10,            // bounds-checking build: a store or a scratch access fell outside its buffer
   DEV_BAD_POSITION = 11,      // a token's position lies outside the rotation tables
-  DEV_BAD_SMEM = 12,          // shared memory or TMEM does not start where a kernel's layout needs it
+  DEV_BAD_SMEM = 12,          // shared memory does not start where a kernel's layout needs it
 };
 
 // Bounds-checking build (-DKCG_DEBUG_BOUNDS; the sanitizer tools are not available everywhere): every

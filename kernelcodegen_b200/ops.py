@@ -3,7 +3,9 @@
 Names follow the reference's Frontend operators (include/Frontend/Operators.h:73-98):
 `matmul` (+ fused `relu`, the `@fuse_matmul_relu` graph of README.md:9-26 with the ReLU of
 src/Frontend/Operators.cc:232-244 folded into the epilogue) and `fmha`
-(BatchedMatmul(Q, K^T) -> Softmax -> BatchedMatmul(P, V), test/test.cc:88-90).
+(BatchedMatmul(Q, K^T) -> Softmax -> BatchedMatmul(P, V), test/test.cc:88-90).  `fmha_with_lse`,
+`fmha_backward`, `qk_norm_rope` and `qk_norm_rope_backward`, what training and serving with that attention need
+beside it, have no counterpart there.
 
 torch is used for device memory and streams only; the arithmetic is done by the hand-written
 sm_100a kernels behind the C-ABI.  Nothing here falls back to torch math.

@@ -4,9 +4,9 @@
 //   delta_i = dO_i.O_i,  dS_ij = P_ij (dO_i.v_j - delta_i)
 //   dV_j = sum_i P_ij dO_i    dK_j = scale sum_i dS_ij q_i    dQ_i = scale sum_j dS_ij k_j
 //
-// dK and dV sum over queries, dQ over keys.  One sweep for all three needs dQ added up across CTAs
-// (fp32 atomics whose order, and so whose rounding, differs from run to run, and a 32-bit dQ in
-// memory that costs as much L2 traffic per tile as the tile's four operands).  Here a launch holds
+// dK and dV sum over queries, dQ over keys.  One sweep for all three needs dQ added up across CTAs in a 32-bit buffer
+// (64 KB of L2 traffic per 128 x 128 tile at D = 128, as much as the tile's four operands), by atomics whose order, and so
+// whose rounding, differs from run to run, or in turns that CTAs wait for.  Here a launch holds
 // two kinds of work item instead, each of which owns what it writes:
 //
 //   kv item  128 keys of one key/value head; streams the query tiles of all its query heads:
@@ -47,7 +47,7 @@
 //   q     S: BN        dP: BN         dQ: D    dS: 2 x BN / 2
 //
 // Measured (B200, bf16, causal, D = 128): 32 heads x 8192 1482 us, 927 TFLOP/s of 5 products (1298 of the 7 that
-// run) in short bursts, 1700 us in calls back to back for seconds, where the power limit holds cuBLAS's own
+// run) in short bursts, 1700 to 1750 us in calls back to back for seconds, where the power limit holds cuBLAS's own
 // bf16 products to 1384 TFLOP/s; 16 heads x 4096 209 us.  One issuer instead of two: 1615 and 228 us.
 // D = 64, 2 x 32 heads x 4096 causal: 780 us, 440 TFLOP/s; one CTA per SM with 128-row tiles measures the same
 // within the noise of the clocks.

@@ -231,7 +231,7 @@ def fmha_with_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: f
     projection: `x.view(B, S, heads, D).transpose(1, 2)`); K and V may have fewer heads, Hkv | H, and query
     head h then reads head h // (H // Hkv).  D is 64 or 128.  Any other extent may be zero: with no keys
     O = 0 and lse = -inf.
-    causal: query i sees the keys j <= i + Skv - Sq.  O is contiguous unless `out` is given (not over an
+    scale is positive; causal: query i sees the keys j <= i + Skv - Sq.  O is contiguous unless `out` is given (not over an
     input).  All entries must be finite, those that no query sees too: they take part in the products with
     weight zero; a visible score that overflows float32 makes its row's O and lse NaN.
     Scores, maxima and sums are float32 (2^x good to 3e-6); P is rounded to bfloat16 for its product with V.

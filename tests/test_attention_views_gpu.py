@@ -72,6 +72,26 @@ def test_one_place_of_a_cache_to_another(cuda_device):
     assert torch.equal(cache[:, :, rest], keep[:, :, rest])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,R", [(128, 128), (96, 38)])
+def test_gradients_over_the_inputs(cuda_device, dtype, D, R):
+    """dq and dk written over q and k themselves, rows of a packed projection and of their own."""
+    from kernelcodegen_b200 import ops
+
+    B, S, H, Hk = 2, 531, 7, 3
+    x, w = make((B, S, H + 2 * Hk, D), 1, dtype), make((D,), 2, dtype)
+    q, k, v = (t.transpose(1, 2) for t in x.split([H, Hk, Hk], dim=2))
+    cos, sin = tables(S, R)
+    dyq, dyk, keep = make(q.shape, 3, dtype), make(k.shape, 4, dtype), v.clone()
+    want = ops.qk_norm_rope_backward(dyq, dyk, q, k, cos, sin, q_weight=w, k_weight=w)
+    flat = [q.contiguous(), k.contiguous()]
+    for a, b in (flat, (q, k)):
+        got = ops.qk_norm_rope_backward(dyq, dyk, a, b, cos, sin, q_weight=w, k_weight=w, dq=a, dk=b)
+        for g, t in zip(got, want):
+            assert torch.equal(g, t)
+    assert torch.equal(v, keep) and ops.last_device_status() == 0
+
+
 def test_expanded_tensors_are_refused_by_name(cuda_device):
     from kernelcodegen_b200 import ops
 
